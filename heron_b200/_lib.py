@@ -22,7 +22,7 @@ HB_ERR_SCRATCH = 8
 HB_ERR_STATIC_SCRATCH = 9
 
 # hb_dtype
-HB_F16, HB_F32, HB_S8, HB_U8, HB_S32 = 0, 1, 2, 3, 4
+HB_F16, HB_F32, HB_S8, HB_U8, HB_S32, HB_BF16 = 0, 1, 2, 3, 4, 5
 
 DTYPE_CODES = {
     "float16": HB_F16,
@@ -68,6 +68,19 @@ EXPORTED_SYMBOLS = (
     "hb_plan_bmm",
     "hb_plan_conv2d_nhwc",
     "hb_plan_conv2d_nhwc_packed",
+    "hb_grouped_gemm",
+    "hb_grouped_gemm_dx",
+    "hb_grouped_gemm_dw",
+    "hb_mxfp4_scale_bytes",
+    "hb_quantize_mxfp4",
+    "hb_dequantize_mxfp4",
+    "hb_gemm_mxfp4",
+    "hb_grouped_gemm_mxfp4",
+    "hb_plan_grouped_gemm",
+    "hb_plan_grouped_gemm_dx",
+    "hb_plan_grouped_gemm_dw",
+    "hb_plan_gemm_mxfp4",
+    "hb_plan_grouped_gemm_mxfp4",
     "hb_plan_launch",
     "hb_plan_knobs",
     "hb_plan_set_peer_outputs",
@@ -226,6 +239,21 @@ def load():
     lib.hb_plan_conv2d_nhwc.argtypes = [pp] + lib.hb_conv2d_nhwc.argtypes[:-1]
     lib.hb_plan_conv2d_nhwc_packed.restype = c_int
     lib.hb_plan_conv2d_nhwc_packed.argtypes = [pp] + lib.hb_conv2d_nhwc_packed.argtypes[:-1]
+    for name in ("hb_grouped_gemm", "hb_grouped_gemm_dx", "hb_grouped_gemm_dw"):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = c_int, [c_void_p] * 4 + [c_int] * 4 + [c_int] * 2 + [kp, c_void_p]
+    lib.hb_mxfp4_scale_bytes.restype = c_size_t
+    lib.hb_mxfp4_scale_bytes.argtypes = [c_int] * 4
+    for name in ("hb_quantize_mxfp4", "hb_dequantize_mxfp4"):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = c_int, [c_void_p] * 4 + [c_int] * 4 + [c_int, c_void_p]
+    lib.hb_gemm_mxfp4.restype = c_int
+    lib.hb_gemm_mxfp4.argtypes = [c_void_p] * 5 + [c_int] * 3 + [c_int, kp, c_void_p]
+    lib.hb_grouped_gemm_mxfp4.restype = c_int
+    lib.hb_grouped_gemm_mxfp4.argtypes = [c_void_p] * 6 + [c_int] * 4 + [c_int, kp, c_void_p]
+    for name in ("grouped_gemm", "grouped_gemm_dx", "grouped_gemm_dw", "gemm_mxfp4", "grouped_gemm_mxfp4"):
+        fn = getattr(lib, "hb_plan_" + name)
+        fn.restype, fn.argtypes = c_int, [pp] + getattr(lib, "hb_" + name).argtypes[:-1]
     lib.hb_plan_launch.restype = c_int
     lib.hb_plan_launch.argtypes = [c_void_p, c_void_p]
     lib.hb_plan_knobs.restype = c_int

@@ -1,6 +1,7 @@
 // The C ABI of libheron_b200.so (include/heron_b200.h): every entry point checks its arguments,
 // builds a plan (tensor maps, knobs, launch geometry) and enqueues it, or hands the plan back.
 #include "hb_plan_conv.cuh"
+#include "hb_plan_group.cuh"
 
 extern "C" {
 
@@ -306,6 +307,93 @@ int hb_plan_conv2d_nhwc_packed(hb_plan** plan, const void* in, const void* w_pac
   return new_plan(plan, [&](hb_plan* p) {
     return plan_conv_packed(in, w_packed, out, N, H, W, CI, CO, KH, KW, stride_h, stride_w, pad, pad,
                             dil_h, dil_w, sco, scratch, scratch_bytes, knobs, p);
+  });
+}
+
+// ---- products grouped by expert, 4-bit products, MXFP4 quantisation ----------------------------
+int hb_grouped_gemm(const void* x, const void* w, void* out, const int* offsets, int T, int K, int N, int E,
+                    hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream) {
+  hb_plan plan;
+  const int rc = plan_grouped(hb::kFwd, w, x, out, offsets, T, K, N, E, in, out_t, knobs, &plan);
+  return rc != HB_OK ? rc : run_plan(&plan, static_cast<cudaStream_t>(stream));
+}
+
+int hb_grouped_gemm_dx(const void* dy, const void* w, void* dx, const int* offsets, int T, int K, int N, int E,
+                       hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream) {
+  hb_plan plan;
+  const int rc = plan_grouped(hb::kDx, w, dy, dx, offsets, T, K, N, E, in, out_t, knobs, &plan);
+  return rc != HB_OK ? rc : run_plan(&plan, static_cast<cudaStream_t>(stream));
+}
+
+int hb_grouped_gemm_dw(const void* dy, const void* x, void* dw, const int* offsets, int T, int K, int N, int E,
+                       hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream) {
+  hb_plan plan;
+  const int rc = plan_grouped(hb::kDw, x, dy, dw, offsets, T, K, N, E, in, out_t, knobs, &plan);
+  return rc != HB_OK ? rc : run_plan(&plan, static_cast<cudaStream_t>(stream));
+}
+
+size_t hb_mxfp4_scale_bytes(int batch, int rows, int K, int groups) { return mx_scale_bytes(batch, rows, K, groups); }
+
+int hb_quantize_mxfp4(const void* x, void* codes, void* scales, const int* offsets, int batch, int rows, int K,
+                      int groups, hb_dtype in, void* stream) {
+  return run_mx(false, x, codes, scales, offsets, batch, rows, K, groups, in, static_cast<cudaStream_t>(stream));
+}
+
+int hb_dequantize_mxfp4(const void* codes, const void* scales, void* out, const int* offsets, int batch, int rows,
+                        int K, int groups, hb_dtype out_t, void* stream) {
+  return run_mx(true, out, codes, scales, offsets, batch, rows, K, groups, out_t, static_cast<cudaStream_t>(stream));
+}
+
+int hb_gemm_mxfp4(const void* A, const void* a_scales, const void* B, const void* b_scales, void* C, int M, int K,
+                  int N, hb_dtype out_t, const hb_knobs* knobs, void* stream) {
+  hb_plan plan;
+  const int rc = plan_mx(A, a_scales, B, b_scales, C, nullptr, M, K, N, 1, out_t, knobs, &plan);
+  return rc != HB_OK ? rc : run_plan(&plan, static_cast<cudaStream_t>(stream));
+}
+
+int hb_grouped_gemm_mxfp4(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out,
+                          const int* offsets, int T, int K, int N, int E, hb_dtype out_t, const hb_knobs* knobs,
+                          void* stream) {
+  if (!offsets && T > 0) return HB_ERR_ALIGN;
+  hb_plan plan;
+  const int rc = plan_mx(x, x_scales, w, w_scales, out, offsets, T, K, N, E, out_t, knobs, &plan);
+  return rc != HB_OK ? rc : run_plan(&plan, static_cast<cudaStream_t>(stream));
+}
+
+int hb_plan_grouped_gemm(hb_plan** plan, const void* x, const void* w, void* out, const int* offsets, int T, int K,
+                         int N, int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs) {
+  return new_plan(plan, [&](hb_plan* p) {
+    return plan_grouped(hb::kFwd, w, x, out, offsets, T, K, N, E, in, out_t, knobs, p);
+  });
+}
+
+int hb_plan_grouped_gemm_dx(hb_plan** plan, const void* dy, const void* w, void* dx, const int* offsets, int T, int K,
+                            int N, int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs) {
+  return new_plan(plan, [&](hb_plan* p) {
+    return plan_grouped(hb::kDx, w, dy, dx, offsets, T, K, N, E, in, out_t, knobs, p);
+  });
+}
+
+int hb_plan_grouped_gemm_dw(hb_plan** plan, const void* dy, const void* x, void* dw, const int* offsets, int T, int K,
+                            int N, int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs) {
+  return new_plan(plan, [&](hb_plan* p) {
+    return plan_grouped(hb::kDw, x, dy, dw, offsets, T, K, N, E, in, out_t, knobs, p);
+  });
+}
+
+int hb_plan_gemm_mxfp4(hb_plan** plan, const void* A, const void* a_scales, const void* B, const void* b_scales,
+                       void* C, int M, int K, int N, hb_dtype out_t, const hb_knobs* knobs) {
+  return new_plan(plan, [&](hb_plan* p) {
+    return plan_mx(A, a_scales, B, b_scales, C, nullptr, M, K, N, 1, out_t, knobs, p);
+  });
+}
+
+int hb_plan_grouped_gemm_mxfp4(hb_plan** plan, const void* x, const void* x_scales, const void* w,
+                               const void* w_scales, void* out, const int* offsets, int T, int K, int N, int E,
+                               hb_dtype out_t, const hb_knobs* knobs) {
+  if (!offsets && T > 0) return HB_ERR_ALIGN;
+  return new_plan(plan, [&](hb_plan* p) {
+    return plan_mx(x, x_scales, w, w_scales, out, offsets, T, K, N, E, out_t, knobs, p);
   });
 }
 

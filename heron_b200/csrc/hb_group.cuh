@@ -1,0 +1,519 @@
+// Products grouped by expert, and products of 4-bit microscaled operands (sm_100a).
+//
+// Rows 0..T-1 of a token matrix belong to E groups: group e owns rows offsets[e] .. offsets[e+1]-1
+// (offsets lie in device memory; the host never reads them).  One kernel body, four modes:
+//
+//   kFwd  out[r, n]    = sum_k x[r, k]  * w[e(r), n, k]
+//   kDx   dx[r, k]     = sum_n dy[r, n] * w[e(r), n, k]
+//   kDw   dw[e, n, k]  = sum_{r in e} dy[r, n] * x[r, k]        (zeros for a group without rows)
+//   kMx   kFwd with both operands in MXFP4; with offsets == nullptr one group of all T rows, which is
+//         the dense product C = A * B^T
+//
+// All are D[m, c] = sum_j A[m, j] * B[c, j] with D's M axis on the 128 TMEM lanes.  The M axis is
+// always the contiguous axis of the output (a feature), never the ragged one: a tile's columns are
+// tokens, and the width of an MMA is chosen per tile in steps of 16 (N of tcgen05.mma), so a group of
+// five rows costs a 128 x 16 product and not a 128 x 128 one.  With the roles the other way round a
+// group's last tile would always be computed 128 rows high.  The epilogue thread of lane m then
+// stores its columns one output row at a time: a warp's 32 lanes write 64 or 128 consecutive bytes,
+// whole sectors whatever the extents, so no output extent has an alignment rule.
+//
+//   mode   A (M axis)                     B (columns)              reduction
+//   kFwd   w, K-major                     x, K-major               K
+//   kDx    w, MN-major (k contiguous)     dy, K-major              N
+//   kDw    x, MN-major (k contiguous)     dy, MN-major             the group's rows (ragged)
+//   kMx    w codes, K-major               x codes, K-major         K
+//
+// Operand layouts, the ring of TMA stages, the roles of the warps and the bounded waits are those of
+// hb_umma_kernel (hb_kernel.cuh).  In kDw a group's last block of 64 rows usually reaches into the
+// next group: the MMA warp writes zeros over those rows of both operands (another group's infinity
+// times zero would be NaN) up to the next multiple of 16 and issues no MMA beyond it.
+//
+// Tiles are listed on the device: every CTA reads the offsets, keeps the groups that have rows (all
+// of them in kDw) with a running count of tiles in shared memory, and walks tiles blockIdx.x,
+// blockIdx.x + gridDim.x, ...  A group's rows are cut into equal tiles, not full ones and a rest, so
+// that the tiles of a wave cost about the same.  Offsets are clamped to [0, T] and a group whose end
+// lies before its start counts as empty: wrong offsets give wrong rows, never an access out of range.
+#pragma once
+#include "hb_kernel.cuh"
+#include <cuda_bf16.h>
+
+namespace hb {
+
+enum { kFwd = 0, kDx = 1, kDw = 2, kMx = 3 };
+
+constexpr int kMaxGroups = 1024;
+constexpr int kGroupThreads = 32 * 7;  // A producer, MMA, four epilogue warps, B producer
+constexpr int kSpan = 128;             // bytes of the reduction axis in a ring stage (TMA swizzle span)
+constexpr int kAtomBytes = 512;        // scales of 128 rows x 128 elements
+
+struct GroupParams {
+  const int* offsets;   // E + 1; nullptr: one group of T rows
+  int E, T;
+  int M;                // extent of the M axis (the output's contiguous extent)
+  int C;                // kDw: extent of the column axis; otherwise unused (columns are a group's rows)
+  int R;                // extent of the reduction axis; kDw: unused (a group's rows)
+  int BN;               // widest tile, multiple of 32 (64 in kDw and kMx)
+  int stages, acc_stages, tmem_cols, tiles_m;
+  int out_type;         // 0: fp32, 1: fp16, 2: bf16
+  uint32_t idesc;       // without the N field
+  void* out;
+  long long ldc;        // elements between consecutive output rows
+  long long out_group;  // kDw: elements between the outputs of consecutive groups
+  const uint8_t* sfa;   // kMx: scales of w (per expert) and of the token matrix
+  const uint8_t* sfb;
+  int silent_producer;  // test hook, see hb_knobs
+  long long wait_limit_cycles;
+};
+
+// One group as the walkers see it.
+struct GroupEntry {
+  int e, start, n, end_tile;  // index, first row, rows, one past its last tile
+};
+
+struct GroupTile {
+  int e, start, n;  // group
+  int m0;           // first M index of the (pair) tile
+  int c0, ncols;    // first column within the group (kDw: of the column axis) and valid columns
+  int nmma;         // columns the MMA computes
+  int blocks;       // reduction blocks
+};
+
+__host__ __device__ __forceinline__ int round_up(int v, int step) { return (v + step - 1) / step * step; }
+
+// Column tiles of a group with n rows and the width of all but its last.  Widths are multiples of the
+// MMA's column step; in kMx a tile starts at a multiple of 64 rows of its group (128 where the widest
+// tile is a multiple of 128), because scales lie in tiles of 128 rows.
+template <int MODE, int CG>
+__host__ __device__ __forceinline__ int group_width(int n, int tiles, int BN) {
+  if (tiles <= 1) return BN;
+  const int step = MODE == kMx ? (BN % 128 ? 64 : 128) : 16 * CG;
+  return round_up((n + tiles - 1) / tiles, step);
+}
+
+template <int MODE, int CG>
+__device__ __forceinline__ bool group_tile(const GroupParams& p, const GroupEntry* g, int& at, int t, int total,
+                                           GroupTile& o) {
+  if (t >= total) return false;
+  while (g[at].end_tile <= t) ++at;  // (tiles are taken in ascending order)
+  const GroupEntry ge = g[at];
+  const int first = at ? g[at - 1].end_tile : 0;
+  o.e = ge.e;
+  o.start = ge.start;
+  o.n = ge.n;
+  const int cols = MODE == kDw ? p.C : ge.n;
+  const int ct = (cols + p.BN - 1) / p.BN;
+  const int r = t - first;
+  const int mt = r / ct;
+  o.m0 = mt * kTileM * CG;
+  const int w = MODE == kDw ? p.BN : group_width<MODE, CG>(cols, ct, p.BN);
+  o.c0 = (r - mt * ct) * w;
+  o.ncols = min(w, cols - o.c0);
+  o.nmma = round_up(o.ncols, 16 * CG);
+  constexpr int kElems = MODE == kMx ? 256 : 64;  // reduction elements of a stage
+  const int red = MODE == kDw ? ge.n : p.R;
+  o.blocks = (red + kElems - 1) / kElems;
+  return true;
+}
+
+// Fills the group list; called by all threads, ends behind a barrier.  Returns the tile count.
+template <int MODE, int CG>
+__device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, int* total) {
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    int s = 0, t = p.T;
+    if (p.offsets) {
+      s = min(max(p.offsets[e], 0), p.T);
+      t = min(max(p.offsets[e + 1], s), p.T);
+    }
+    g[e].start = s;
+    g[e].n = t - s;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int kept = 0, sum = 0;
+    for (int base = 0; base < p.E; base += 32) {
+      const int e = base + lane;
+      const int start = e < p.E ? g[e].start : 0, n = e < p.E ? g[e].n : 0;
+      const int cols = MODE == kDw ? (e < p.E ? p.C : 0) : n;
+      int tiles = (cols + p.BN - 1) / p.BN * p.tiles_m;
+      const uint32_t has = __ballot_sync(0xffffffffu, tiles > 0);
+      int incl = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
+      }
+      // (every lane holds its group in registers: the entries written below are at or before these)
+      if (tiles > 0) {
+        const int slot = kept + __popc(has & ((1u << lane) - 1u));
+        g[slot] = GroupEntry{e, start, n, sum + incl};
+      }
+      __syncwarp();
+      kept += __popc(has);
+      sum += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) *total = sum;
+  }
+  __syncthreads();
+  return *total;
+}
+
+struct GroupBars {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int total;
+};
+
+// Bytes of a ring stage of one CTA: operands, and in kMx the scales of 256 elements: one tile row of
+// scales for A, up to two for B's columns.
+__host__ __device__ __forceinline__ int group_sf_rows(int BN) { return BN <= 64 ? 1 : (BN + 127) / 128; }
+template <int MODE, int CG>
+__host__ __device__ __forceinline__ int group_stage_bytes(int BN) {
+  return (kTileM + BN / CG) * kSpan + (MODE == kMx ? (1 + group_sf_rows(BN)) * 2 * kAtomBytes : 0);
+}
+
+template <int MODE, int CG>
+__global__ void __launch_bounds__(kGroupThreads, 1)
+hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmB16, const GroupParams p) {
+  constexpr bool A_MN = MODE == kDx || MODE == kDw;
+  constexpr bool B_MN = MODE == kDw;
+  constexpr int kElems = MODE == kMx ? 256 : 64;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t cta_rank = (CG == 2) ? cluster_ctarank() : 0u;
+  const bool leader = cta_rank == 0u;
+  constexpr int a_bytes = kTileM * kSpan;
+  const int b_bytes = p.BN / CG * kSpan;
+  const int sf_rows = group_sf_rows(p.BN);
+  const int sf_bytes = MODE == kMx ? (1 + sf_rows) * 2 * kAtomBytes : 0;  // A's tile row first, then B's
+  const uint32_t sA = smem_base;
+  const uint32_t sB = sA + p.stages * a_bytes;
+  const uint32_t sSF = sB + p.stages * b_bytes;
+  uint8_t* after = smem + (sSF - smem_base) + p.stages * sf_bytes;
+  GroupBars* bars = reinterpret_cast<GroupBars*>(after);
+  GroupEntry* groups = reinterpret_cast<GroupEntry*>(after + ((sizeof(GroupBars) + 15) & ~15));
+  volatile int* abort_flag = &bars->abort_flag;
+  const WaitCtx wctx{abort_flag, p.wait_limit_cycles > 0 ? p.wait_limit_cycles : HB_WAIT_LIMIT_CYCLES};
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&bars->full[s]), 1);
+      mbar_init(smem_u32(&bars->empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&bars->tmem_full[a]), 1);
+      mbar_init(smem_u32(&bars->tmem_empty[a]), 4 * CG);
+    }
+    mbar_init(smem_u32(&bars->drain), 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) tmem_alloc_cg<CG>(smem_u32(&bars->tmem_base), static_cast<uint32_t>(p.tmem_cols));
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  griddep_wait();  // (the offsets too may come from the kernel before)
+  griddep_launch_dependents();
+  const int total = group_list<MODE, CG>(p, groups, &bars->total);
+  const int first_tile = blockIdx.x / CG;
+  const int tile_step = gridDim.x / CG;
+
+  // B rows (K-major) or columns (MN-major) of a tile that this CTA stages, and how they are fetched
+  // (boxes of 16 rows for narrow tiles, of 64 otherwise)
+  auto b_boxes = [&](int nmma, int& box) {
+    const int mine = nmma / CG;
+    box = (!B_MN && mine <= 48) ? 16 : 64;
+    return (mine + box - 1) / box;
+  };
+  auto sf_b_rows = [&](const GroupTile& tl) { return ((tl.c0 & 127) + tl.nmma + 127) >> 7; };
+
+  // part bit 0: A (and the barrier's byte count); bit 1: B
+  auto produce = [&](int part) {
+    int stage = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    int at = 0;
+    GroupTile tl;
+    const int kt = MODE == kMx ? (p.R + 127) / 128 : 0;  // scale tiles along the reduction
+    for (int t = first_tile; ok && !p.silent_producer && group_tile<MODE, CG>(p, groups, at, t, total, tl);
+         t += tile_step) {
+      int box;
+      const int boxes = b_boxes(tl.nmma, box);
+      const uint32_t tx_ab = static_cast<uint32_t>(a_bytes + boxes * box * kSpan) * CG;
+      const int nb_sf = MODE == kMx ? sf_b_rows(tl) : 0;
+      const int m0 = tl.m0 + static_cast<int>(cta_rank) * kTileM;
+      const int mine0 = tl.c0 + static_cast<int>(cta_rank) * (tl.nmma / CG);  // first B row / column
+      const uint8_t* sfa = nullptr;
+      const uint8_t* sfb = nullptr;
+      if (MODE == kMx) {
+        sfa = p.sfa + (static_cast<long long>(tl.e) * p.tiles_m + tl.m0 / kTileM) * kt * kAtomBytes;
+        sfb = p.sfb + (static_cast<long long>(tl.start / 128 + tl.e + tl.c0 / 128)) * kt * kAtomBytes;
+      }
+      for (int kb = 0; kb < tl.blocks; ++kb) {
+        const uint32_t full_local = smem_u32(&bars->full[stage]);
+        const uint32_t full = (CG == 2) ? mapa(full_local, 0) : full_local;
+        if (!mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, wctx)) {
+          ok = false;
+          break;
+        }
+        const uint32_t sf_tile = MODE == kMx ? min(2, kt - 2 * kb) * kAtomBytes : 0;
+        if (leader && (part & 1)) mbar_arrive_expect_tx(full_local, tx_ab + (1 + nb_sf) * sf_tile);
+        const uint32_t dA = sA + stage * a_bytes, dB = sB + stage * b_bytes, dSF = sSF + stage * sf_bytes;
+        // first index of this block on the reduction axis (in bytes of packed codes for kMx)
+        const int red = MODE == kMx ? kb * kSpan : kb * kElems;
+        if (part & 1) {
+          if (MODE == kFwd || MODE == kMx) {
+            tma_load_3d_cg<CG>(dA, &tmA, full, red, m0, tl.e);
+          } else {
+            const int row = MODE == kDw ? tl.start + red : red;
+            const int z = MODE == kDw ? 0 : tl.e;
+            tma_load_3d_cg<CG>(dA, &tmA, full, m0, row, z);
+            tma_load_3d_cg<CG>(dA + a_bytes / 2, &tmA, full, m0 + 64, row, z);
+          }
+          if (MODE == kMx) bulk_load(dSF, sfa + static_cast<long long>(kb) * 2 * kAtomBytes, sf_tile, full);
+        }
+        if (part & 2) {
+          const CUtensorMap* tb = box == 16 ? &tmB16 : &tmB;
+          for (int i = 0; i < boxes; ++i) {
+            if (B_MN)
+              tma_load_3d_cg<CG>(dB + i * 64 * kSpan, tb, full, mine0 + i * 64, tl.start + red, 0);
+            else
+              tma_load_3d_cg<CG>(dB + i * box * kSpan, tb, full, red, tl.start + mine0 + i * box, 0);
+          }
+          for (int i = 0; i < nb_sf; ++i)
+            bulk_load(dSF + (1 + i) * 2 * kAtomBytes,
+                      sfb + (static_cast<long long>(i) * kt + 2 * kb) * kAtomBytes, sf_tile, full);
+        }
+        ++issued;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok) {  // wait (bounded) for the copies in flight; see hb_umma_kernel
+      if (leader) {
+        const int pending = issued < p.stages ? static_cast<int>(issued) : p.stages;
+        for (int i = 0; i < pending; ++i) {
+          if (--stage < 0) {
+            stage = p.stages - 1;
+            phase ^= 1u;
+          }
+          mbar_wait_drain(smem_u32(&bars->full[stage]), phase);
+        }
+      } else {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000LL) {
+        }
+      }
+    }
+  };
+
+  // The MMA role.  One elected lane issues; in kDw the whole warp walks along, to write the zeros
+  // behind a group's last row.
+  auto multiply = [&](bool issue) {
+    int stage = 0;
+    uint32_t phase = 0;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    auto all_lanes = [](bool v) { return MODE == kDw ? __all_sync(0xffffffffu, v) != 0 : v; };
+    constexpr uint32_t layout_type = 2u;  // 128-byte swizzle
+    constexpr uint64_t desc_hi = static_cast<uint64_t>(((8u * kSpan) >> 4) | (1u << 14) | (layout_type << 29)) << 32;
+    // MN-major: 64 x 64 chunks of 8 KB, 16 reduction rows (2 KB) per MMA; K-major: 32 bytes per MMA
+    constexpr uint32_t chunk16 = 64u * kSpan >> 4;
+    constexpr uint32_t a_lo_fixed = (A_MN ? chunk16 : 1u) << 16, b_lo_fixed = (B_MN ? chunk16 : 1u) << 16;
+    constexpr uint32_t a_step = A_MN ? 16u * kSpan >> 4 : 2u, b_step = B_MN ? 16u * kSpan >> 4 : 2u;
+    const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
+    const uint32_t sf_cols = static_cast<uint32_t>(8 * (1 + sf_rows));  // TMEM columns of a stage's scales
+    const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
+    int at = 0;
+    GroupTile tl;
+    for (int t = first_tile; ok && group_tile<MODE, CG>(p, groups, at, t, total, tl); t += tile_step) {
+      if (MODE == kDw && tl.blocks == 0) continue;  // (the epilogue writes zeros without an accumulator)
+      ok = all_lanes(mbar_wait(smem_u32(&bars->tmem_empty[acc]), acc_phase ^ 1u, wctx));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * p.BN);
+      const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tl.nmma >> 3) << 17);
+      uint32_t accum = 0u;
+      const int nb_sf = MODE == kMx ? sf_b_rows(tl) : 0;
+      for (int kb = 0; kb < tl.blocks; ++kb) {
+        ok = all_lanes(mbar_wait(full0 + 8u * stage, phase, wctx));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t stA = sA + stage * a_bytes, stB = sB + stage * b_bytes;
+        // MMAs of this stage: 16 (kMx: 64) reduction elements each
+        int steps = 4;
+        if (MODE == kMx) steps = min(4, (p.R - kb * kElems + 63) / 64);
+        if (MODE == kDw) {
+          const int valid = min(64, tl.n - kb * 64);
+          if (valid < 64) {
+            steps = (valid + 15) / 16;
+            const int chunks = 2 + (tl.nmma + 63) / 64;
+            const int vecs = (steps * 16 - valid) * 8;  // 16-byte vectors of a 64-column chunk
+            for (int c = 0; c < chunks; ++c) {
+              const uint32_t base = (c < 2 ? stA + c * 64 * kSpan : stB + (c - 2) * 64 * kSpan) + valid * kSpan;
+              for (int v = lane; v < vecs; v += 32)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + v * 16), "r"(0) : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (issue) {
+          const uint32_t a_lo = ((stA >> 4) & 0x3FFFu) | a_lo_fixed, b_lo = ((stB >> 4) & 0x3FFFu) | b_lo_fixed;
+          uint32_t ta = 0, tb = 0;
+          if constexpr (MODE == kMx) {
+            // scales into TMEM.  A stage has its own columns: they are written again only after the
+            // MMAs that read them have freed the stage.  Columns: A's two tiles of 128 elements, then
+            // per tile of 128 elements B's tile rows side by side (column j holds rows 32 j ...).
+            ta = sf_tmem + stage * sf_cols;
+            tb = ta + 8u;
+            const uint32_t sf = sSF + stage * sf_bytes;
+            const int tiles_k = min(2, (p.R - kb * kElems + 127) / 128);
+            for (int ka = 0; ka < tiles_k; ++ka) {
+              tmem_cp_scales(ta + 4u * ka, sf + ka * kAtomBytes);
+              for (int i = 0; i < nb_sf; ++i)
+                tmem_cp_scales(tb + static_cast<uint32_t>(ka * 4 * sf_rows + 4 * i), sf + ((1 + i) * 2 + ka) * kAtomBytes);
+            }
+            tb += static_cast<uint32_t>((tl.c0 & 127) >> 5);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k < steps) {
+              const uint64_t ad = desc_hi | (a_lo + a_step * k), bd = desc_hi | (b_lo + b_step * k);
+              if constexpr (MODE == kMx)
+                umma_mxf4(d_tmem, ad, bd, idesc | (k & 1 ? (2u << 4) | (2u << 29) : 0u), ta + 4u * (k >> 1),
+                          tb + static_cast<uint32_t>(4 * sf_rows * (k >> 1)), accum);
+              else
+                umma_cg<CG, 0>(d_tmem, ad, bd, idesc, accum);
+              accum = 1u;
+            }
+          }
+          umma_commit_cg<CG>(empty0 + 8u * stage);
+        }
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if (issue) umma_commit_cg<CG>(smem_u32(&bars->tmem_full[acc]));
+      if (++acc == p.acc_stages) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if (!ok && issue) {
+      umma_commit_local<CG>(smem_u32(&bars->drain));
+      mbar_wait_drain(smem_u32(&bars->drain), 0u);
+    }
+  };
+
+  if (warp == 0) {
+    if (elect_one()) produce(1);
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader) {
+      if (MODE == kDw) {
+        const bool one = elect_one();
+        multiply(one);
+      } else if (elect_one()) {
+        multiply(true);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    if (elect_one()) produce(2);
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    int at = 0;
+    GroupTile tl;
+    for (int t = first_tile; group_tile<MODE, CG>(p, groups, at, t, total, tl); t += tile_step) {
+      const bool empty = MODE == kDw && tl.blocks == 0;
+      const int m = tl.m0 + static_cast<int>(cta_rank) * kTileM + q * 32 + lane;
+      const bool mine = m < p.M;
+      const long long row0 = MODE == kDw ? tl.c0 : static_cast<long long>(tl.start) + tl.c0;
+      const long long first = (MODE == kDw ? tl.e * p.out_group : 0) + row0 * p.ldc + m;
+      if (!empty) {
+        if (!mbar_wait_relaxed(smem_u32(&bars->tmem_full[acc]), acc_phase, wctx)) break;
+        tc_fence_after();
+      }
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * p.BN);
+      for (int c = 0; c < tl.ncols; c += 32) {
+        uint32_t v[32];
+        if (empty) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0u;
+        } else {
+          tmem_ld_32x32(t_addr + c, v);
+          tmem_ld_wait();
+          if (c + 32 >= tl.ncols) {  // last read of this accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (CG == 2)
+                mbar_arrive_cluster(mapa(smem_u32(&bars->tmem_empty[acc]), 0));
+              else
+                mbar_arrive(smem_u32(&bars->tmem_empty[acc]));
+            }
+          }
+        }
+        if (mine) {
+          const int left = tl.ncols - c;
+          const long long o = first + c * p.ldc;
+          if (p.out_type == 0) {
+            float* out = static_cast<float*>(p.out) + o;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) out[j * p.ldc] = __uint_as_float(v[j]);
+          } else if (p.out_type == 1) {
+            __half* out = static_cast<__half*>(p.out) + o;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) out[j * p.ldc] = __float2half_rn(__uint_as_float(v[j]));
+          } else {
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + o;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) out[j * p.ldc] = __float2bfloat16_rn(__uint_as_float(v[j]));
+          }
+        }
+      }
+      if (!empty && ++acc == p.acc_stages) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_cg<CG>(tmem_base, static_cast<uint32_t>(p.tmem_cols));
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_hb_status, kErrTimeout);
+}
+
+}  // namespace hb

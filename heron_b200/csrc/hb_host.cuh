@@ -9,6 +9,8 @@
 #include "hb_glue.cuh"
 #include "hb_conv_strip.cuh"
 #include "hb_conv_strip_t.cuh"
+#include "hb_group.cuh"
+#include "hb_mx.cuh"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -55,7 +57,13 @@ bool setup_device(Driver* d) {
   if (prop.major != 10) return false;
   d->sm_count = prop.multiProcessorCount;
   // Opt in to the large dynamic shared-memory carve-out for every kernel instantiation.
-  const void* kernels[31] = {
+  const void* kernels[37] = {
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 2>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kDx, 1>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kDx, 2>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kDw, 1>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 1>),
       reinterpret_cast<const void*>(&hb::hb_conv_strip_t_kernel<2>),
       reinterpret_cast<const void*>(&hb::hb_conv_strip_t_kernel<4>),
       reinterpret_cast<const void*>(&hb::hb_umma_kernel<4, 1, 0, 1>),
@@ -134,6 +142,7 @@ int esize(hb_dtype t) {
     case HB_S8: return 1;
     case HB_U8: return 1;
     case HB_S32: return 4;
+    case HB_BF16: return 2;
   }
   return 0;
 }
@@ -157,6 +166,7 @@ CUtensorMapDataType tmap_dtype(hb_dtype t) {
     case HB_F16: return CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     case HB_F32: return CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     case HB_S32: return CU_TENSOR_MAP_DATA_TYPE_INT32;
+    case HB_BF16: return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     default: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
   }
 }
@@ -378,6 +388,12 @@ struct hb_plan {
   // wide strip conv (conv_algo 3): channels on the MMA's M axis, up to 256 pixels on N
   bool strip_t;
   hb::StripTParams spt;
+  // products grouped by expert and 4-bit products: tmA, tmB (64-row boxes), tmB2 (16-row boxes);
+  // group_zero_bytes: no rows at all, the weight gradient is cleared and nothing is launched
+  bool group;
+  int group_mode;
+  hb::GroupParams gp;
+  size_t group_zero_bytes;
   // NCHW operators only: one launch that brings input and filter to NHWC / HWIO first (the conv
   // kernel's epilogue writes NCHW itself)
   bool has_pre, pre_is_stem;

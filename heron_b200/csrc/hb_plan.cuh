@@ -331,7 +331,10 @@ int run_plan(const hb_plan* plan, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
+int run_group(const hb_plan* plan, cudaStream_t stream);  // (hb_plan_group.cuh)
+
 int run_main(const hb_plan* plan, cudaStream_t stream) {
+  if (plan->group) return run_group(plan, stream);
   if (plan->scan_b) {
     if (plan->scan_es == 2)
       hb::hb_scan_mask_kernel<uint16_t><<<plan->scan_blocks, 256, 0, stream>>>(
@@ -478,7 +481,7 @@ int plan_scan(const void* A, void* out, int M, int N, int K, hb_dtype in_a, hb_d
 // GPUs' output buffers, mapped into this process).  n = 0 takes them away again.
 int set_peer_outputs(hb_plan* plan, int n, void* const* outs) {
   if (!plan || n < 0 || n > 15 || (n > 0 && !outs)) return HB_ERR_SHAPE;
-  if (plan->strip || plan->strip_t || !plan->p.epilogue || plan->p.kslab || plan->p.ksplit > 1 || plan->p.sk ||
+  if (plan->group || plan->strip || plan->strip_t || !plan->p.epilogue || plan->p.kslab || plan->p.ksplit > 1 || plan->p.sk ||
       plan->has_post)
     return HB_ERR_KNOB;
   Driver& d = driver();

@@ -1,0 +1,274 @@
+// Plans for the products grouped by expert and the 4-bit products (hb_group.cuh), and the launches of
+// the quantisation kernels (hb_mx.cuh).
+#pragma once
+#include "hb_plan.cuh"
+
+namespace {
+
+int out_type_of(hb_dtype t) { return t == HB_F32 ? 0 : (t == HB_F16 ? 1 : (t == HB_BF16 ? 2 : -1)); }
+
+struct GroupProblem {
+  int mode;  // hb::kFwd ...
+  int T, E;  // rows of the token matrix, groups
+  int M, C, R;  // see hb::GroupParams
+  hb_dtype in, out;  // in: unused for kMx
+};
+
+int group_fixed_smem(int E) {
+  return 1024 /*alignment of the ring*/ + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
+         E * static_cast<int>(sizeof(hb::GroupEntry));
+}
+
+int group_stage(const GroupProblem& g, int BN, int cg) {
+  if (g.mode == hb::kMx) return hb::group_stage_bytes<hb::kMx, 1>(BN);
+  return cg == 2 ? hb::group_stage_bytes<hb::kFwd, 2>(BN) : hb::group_stage_bytes<hb::kFwd, 1>(BN);
+}
+
+int group_tmem(const GroupProblem& g, const hb_knobs& k) {
+  int c = k.acc_stages * k.tile_n;
+  if (g.mode == hb::kMx) c += k.stages * 8 * (1 + hb::group_sf_rows(k.tile_n));
+  return c;
+}
+
+void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
+  hb_knobs k;
+  if (in) k = *in; else std::memset(&k, 0, sizeof(k));
+  const int avg = g.T / g.E;  // mean rows of a group
+  if (k.cta_group == 0)
+    k.cta_group = ((g.mode == hb::kFwd || g.mode == hb::kDx) && avg >= 256 && g.M >= 256 && k.tile_n % 128 == 0) ? 2 : 1;
+  if (k.tile_n == 0) {
+    if (g.mode == hb::kDw)
+      k.tile_n = g.C > 128 ? 256 : (g.C > 64 ? 128 : 64);
+    else if (g.mode == hb::kMx)
+      k.tile_n = avg > 128 ? 192 : (avg > 48 ? 128 : 64);
+    else
+      k.tile_n = k.cta_group == 2 || avg > 96 ? 256 : (avg > 48 ? 128 : 64);
+  }
+  const int room = kSmemLimit - group_fixed_smem(g.E);
+  if (k.stages == 0) {
+    k.stages = room / group_stage(g, k.tile_n, k.cta_group);
+    const int most = g.mode == hb::kMx ? (512 - k.tile_n) / (8 * (1 + hb::group_sf_rows(k.tile_n))) : hb::kMaxStages;
+    if (k.stages > most) k.stages = most;
+    if (k.stages > hb::kMaxStages) k.stages = hb::kMaxStages;
+    if (k.stages < 1) k.stages = 1;
+  }
+  if (k.acc_stages == 0) {
+    k.acc_stages = 2;
+    if (group_tmem(g, k) > 512) k.acc_stages = 1;
+  }
+  *out = k;
+}
+
+int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
+  if (k.cta_group != 1 && k.cta_group != 2) return HB_ERR_KNOB;
+  if (k.cta_group == 2 && g.mode != hb::kFwd && g.mode != hb::kDx) return HB_ERR_KNOB;
+  // B is fetched in boxes of 64 rows (16 for narrow tiles): a CTA's share of a tile holds whole boxes
+  const int step = k.cta_group == 2 ? 128 : 64;
+  if (k.tile_n < step || k.tile_n > 256 || k.tile_n % step != 0) return HB_ERR_KNOB;
+  if (k.stages < 1 || k.stages > hb::kMaxStages) return HB_ERR_KNOB;
+  if (k.acc_stages < 1 || k.acc_stages > 2) return HB_ERR_KNOB;
+  if (k.max_ctas < 0) return HB_ERR_KNOB;
+  if (group_tmem(g, k) > 512) return HB_ERR_KNOB;
+  if (group_fixed_smem(g.E) + k.stages * group_stage(g, k.tile_n, k.cta_group) > kSmemLimit) return HB_ERR_KNOB;
+  return HB_OK;
+}
+
+// A: w (kFwd, kDx, kMx) or x (kDw); B: the token matrix (kDw: dy).
+int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, const void* sfa, const void* sfb,
+               const int* offsets, const hb_knobs* knobs, hb_plan* plan) {
+  std::memset(plan, 0, sizeof(*plan));
+  plan->group = true;
+  plan->group_mode = g.mode;
+  const int eo = esize(g.out);
+  const bool dw = g.mode == hb::kDw, mx = g.mode == hb::kMx;
+  if (g.T == 0) {  // no rows: nothing to compute, and the gradient of every weight is zero
+    if (!dw) return HB_OK;
+    if (!out || !aligned16(out)) return HB_ERR_ALIGN;
+    Driver& d0 = driver();
+    if (d0.status != HB_OK) return d0.status;
+    plan->gp.out = out;
+    plan->group_zero_bytes = static_cast<size_t>(g.E) * g.M * g.C * eo;
+    return HB_OK;
+  }
+  if (!A || !B || !out || !aligned16(A) || !aligned16(B) || !aligned16(out)) return HB_ERR_ALIGN;
+  if (mx && (!sfa || !sfb || !aligned16(sfa) || !aligned16(sfb))) return HB_ERR_ALIGN;
+  if (!offsets && !(mx && g.E == 1)) return HB_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) return HB_ERR_ALIGN;
+  Driver& d = driver();
+  if (d.status != HB_OK) return d.status;
+  hb_knobs k;
+  group_knobs(g, knobs, &k);
+  int rc = check_group_knobs(g, k);
+  if (rc != HB_OK) return rc;
+
+  hb::GroupParams& p = plan->gp;
+  p.offsets = offsets;
+  p.E = g.E; p.T = g.T; p.M = g.M; p.C = g.C; p.R = g.R;
+  p.BN = k.tile_n; p.stages = k.stages; p.acc_stages = k.acc_stages;
+  p.tmem_cols = next_pow2_cols(group_tmem(g, k));
+  const int rows_m = hb::kTileM * k.cta_group;
+  p.tiles_m = (g.M + rows_m - 1) / rows_m;
+  p.out = out;
+  p.out_type = out_type_of(g.out);
+  p.ldc = g.M;
+  p.out_group = static_cast<long long>(g.C) * g.M;
+  p.sfa = static_cast<const uint8_t*>(sfa);
+  p.sfb = static_cast<const uint8_t*>(sfb);
+  p.silent_producer = k.silent_producer ? 1 : 0;
+  if (p.silent_producer) p.wait_limit_cycles = 200000000LL;
+  // instruction descriptor: M / 16 in bits 24..28, the majors in bits 15 and 16, formats in 7..9 and 10..12
+  p.idesc = static_cast<uint32_t>(rows_m >> 4) << 24;
+  if (mx) {
+    p.idesc |= (1u << 7) | (1u << 10) | (1u << 23);  // E2M1 both, scales E8M0
+  } else {
+    const uint32_t f = g.in == HB_BF16 ? 1u : 0u;
+    p.idesc |= (1u << 4) | (f << 7) | (f << 10);  // fp32 accumulator
+    if (g.mode != hb::kFwd) p.idesc |= 1u << 15;
+    if (dw) p.idesc |= 1u << 16;
+  }
+  // most tiles the offsets can ask for
+  const long long ct = dw ? static_cast<long long>(g.E) * ((g.C + k.tile_n - 1) / k.tile_n)
+                          : (g.T < g.T / k.tile_n + g.E ? g.T : g.T / k.tile_n + g.E);
+  const long long tiles = ct * p.tiles_m;
+  if (tiles > 0x3fffffffLL) return HB_ERR_SHAPE;
+  int units = d.sm_count / k.cta_group;
+  if (k.max_ctas > 0 && k.max_ctas / k.cta_group < units) units = k.max_ctas / k.cta_group;
+  if (units < 1) units = 1;
+  plan->grid = static_cast<int>(tiles < units ? tiles : units) * k.cta_group;
+  plan->smem = group_fixed_smem(g.E) + k.stages * group_stage(g, k.tile_n, k.cta_group);
+  plan->knobs = k;
+
+  const uint64_t T = g.T, E = g.E, M = g.M, R = g.R, C = g.C;
+  if (mx) {
+    const uint64_t row = R / 2;
+    rc = encode_tiled3(d, &plan->tmA, HB_U8, A, row, M, E, row, row * M, 128, hb::kTileM, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, HB_U8, B, row, T, 1, row, row * T, 128, 64, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB2, HB_U8, B, row, T, 1, row, row * T, 128, 16, 128);
+  } else if (dw) {
+    rc = encode_tiled3(d, &plan->tmA, g.in, A, M, T, 1, M * 2, M * 2 * T, 64, 64, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, g.in, B, C, T, 1, C * 2, C * 2 * T, 64, 64, 128);
+    plan->tmB2 = plan->tmB;
+  } else {
+    rc = g.mode == hb::kFwd ? encode_tiled3(d, &plan->tmA, g.in, A, R, M, E, R * 2, R * 2 * M, 64, hb::kTileM, 128)
+                            : encode_tiled3(d, &plan->tmA, g.in, A, M, R, E, M * 2, M * 2 * R, 64, 64, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, g.in, B, R, T, 1, R * 2, R * 2 * T, 64, 64, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB2, g.in, B, R, T, 1, R * 2, R * 2 * T, 64, 16, 128);
+  }
+  return rc;
+}
+
+int plan_grouped(int mode, const void* A, const void* B, void* out, const int* offsets, int T, int K, int N, int E,
+                 hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, hb_plan* plan) {
+  std::memset(plan, 0, sizeof(*plan));
+  if (T < 0 || K <= 0 || N <= 0 || E <= 0 || E > hb::kMaxGroups) return HB_ERR_SHAPE;
+  if ((in != HB_F16 && in != HB_BF16) || out_type_of(out_t) < 0) return HB_ERR_DTYPE;
+  // row pitches of the operands are multiples of 16 bytes (the output's need not be)
+  if (K % 8 != 0 || (mode != hb::kFwd && N % 8 != 0)) return HB_ERR_SHAPE;
+  GroupProblem g;
+  g.mode = mode; g.T = T; g.E = E; g.in = in; g.out = out_t;
+  g.M = mode == hb::kFwd ? N : K;
+  g.C = N;
+  g.R = mode == hb::kFwd ? K : N;
+  return plan_group(g, A, B, out, nullptr, nullptr, offsets, knobs, plan);
+}
+
+int plan_mx(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, const int* offsets,
+            int T, int K, int N, int E, hb_dtype out_t, const hb_knobs* knobs, hb_plan* plan) {
+  std::memset(plan, 0, sizeof(*plan));
+  if (T < 0 || K <= 0 || N <= 0 || E <= 0 || E > hb::kMaxGroups || K % 32 != 0) return HB_ERR_SHAPE;
+  if (out_type_of(out_t) < 0) return HB_ERR_DTYPE;
+  GroupProblem g;
+  g.mode = hb::kMx; g.T = T; g.E = E; g.in = HB_U8; g.out = out_t;
+  g.M = N; g.C = 0; g.R = K;
+  return plan_group(g, w, x, out, w_scales, x_scales, offsets, knobs, plan);
+}
+
+template <int MODE, int CG>
+int launch_group(const hb_plan* plan, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(plan->grid);
+  cfg.blockDim = dim3(hb::kGroupThreads);
+  cfg.dynamicSmemBytes = plan->smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG>, plan->tmA, plan->tmB, plan->tmB2, plan->gp);
+  return e == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+}
+
+int run_group(const hb_plan* plan, cudaStream_t stream) {
+  if (plan->group_zero_bytes)
+    return cudaMemsetAsync(plan->gp.out, 0, plan->group_zero_bytes, stream) == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+  if (plan->grid == 0) return HB_OK;  // no rows
+  const bool pair = plan->knobs.cta_group == 2;
+  switch (plan->group_mode) {
+    case hb::kFwd: return pair ? launch_group<hb::kFwd, 2>(plan, stream) : launch_group<hb::kFwd, 1>(plan, stream);
+    case hb::kDx: return pair ? launch_group<hb::kDx, 2>(plan, stream) : launch_group<hb::kDx, 1>(plan, stream);
+    case hb::kDw: return launch_group<hb::kDw, 1>(plan, stream);
+    default: return launch_group<hb::kMx, 1>(plan, stream);
+  }
+}
+
+// ---- MXFP4 quantisation -----------------------------------------------------------------------
+size_t mx_scale_bytes(int batch, int rows, int K, int groups) {
+  if (batch <= 0 || rows < 0 || K <= 0 || K % 32 != 0 || groups < 0 || groups > hb::kMaxGroups) return 0;
+  if (groups > 0 && batch != 1) return 0;
+  const long long tile_rows = groups > 0 ? rows / 128 + groups : (rows + 127LL) / 128;
+  return static_cast<size_t>(batch) * tile_rows * ((K + 127LL) / 128) * hb::kAtomBytes;
+}
+
+// Both directions: `values` is the input of the quantisation or the output of the way back.
+int run_mx(bool back, const void* values, const void* codes, const void* scales, const int* offsets, int batch,
+           int rows, int K, int groups, hb_dtype type, cudaStream_t stream) {
+  if (batch <= 0 || rows < 0 || K <= 0 || K % 32 != 0 || groups < 0 || groups > hb::kMaxGroups) return HB_ERR_SHAPE;
+  if (groups > 0 && batch != 1) return HB_ERR_SHAPE;
+  const int t = out_type_of(type);
+  if (t < 0) return HB_ERR_DTYPE;
+  if (rows == 0) return HB_OK;
+  if (!values || !codes || !scales || !aligned16(values) || !aligned16(codes) || !aligned16(scales)) return HB_ERR_ALIGN;
+  if ((groups > 0) != (offsets != nullptr) || (reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) return HB_ERR_ALIGN;
+  if (static_cast<long long>(batch) * rows > 0x7fffffffLL) return HB_ERR_SHAPE;
+  Driver& d = driver();
+  if (d.status != HB_OK) return d.status;
+  hb::MxParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = values;
+  p.out = const_cast<void*>(values);
+  p.codes = static_cast<uint8_t*>(const_cast<void*>(codes));
+  p.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  p.offsets = offsets;
+  p.batch = batch; p.rows = rows; p.K = K; p.groups = groups;
+  p.matrix_scales = static_cast<long long>(mx_scale_bytes(1, rows, K, groups));
+  const long long units = static_cast<long long>(batch) * rows * ((K + 127) / 128);
+  const long long blocks = (units + hb::kMxThreads / 16 - 1) / (hb::kMxThreads / 16);
+  const long long cap = static_cast<long long>(d.sm_count) * 8;
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks < cap ? blocks : cap));
+  cfg.blockDim = dim3(hb::kMxThreads);
+  cfg.dynamicSmemBytes = groups > 0 ? (groups + 1) * sizeof(int) : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (back)
+    e = t == 0 ? cudaLaunchKernelEx(&cfg, hb::hb_dequantize_mxfp4_kernel<0>, p)
+               : (t == 1 ? cudaLaunchKernelEx(&cfg, hb::hb_dequantize_mxfp4_kernel<1>, p)
+                         : cudaLaunchKernelEx(&cfg, hb::hb_dequantize_mxfp4_kernel<2>, p));
+  else
+    e = t == 0 ? cudaLaunchKernelEx(&cfg, hb::hb_quantize_mxfp4_kernel<0>, p)
+               : (t == 1 ? cudaLaunchKernelEx(&cfg, hb::hb_quantize_mxfp4_kernel<1>, p)
+                         : cudaLaunchKernelEx(&cfg, hb::hb_quantize_mxfp4_kernel<2>, p));
+  return e == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+}
+
+}  // namespace

@@ -536,3 +536,274 @@ def plan_conv3d_ncdhw(x, w, stride=1, padding=0, out=None, out_dtype=None, scrat
                                           scratch.numel(), _knobs(knobs))
     _lib.check(rc, "hb_plan_conv3d_ncdhw")
     return Plan(h, (x, w, scratch), out)
+
+
+# ---- products grouped by expert --------------------------------------------------------------
+# (types of these operators and of the 4-bit ones only: the operators above keep refusing bfloat16)
+_WIDE_CODES = {torch.float16: _lib.HB_F16, torch.bfloat16: _lib.HB_BF16, torch.float32: _lib.HB_F32}
+
+# The small calls of these operators are bound by the host (a token's product takes the GPU a few
+# microseconds): one pass over the checks, addresses and streams as plain ints.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _wide_code(dtype):
+    code = _WIDE_CODES.get(dtype)
+    if code is None:
+        raise _lib.HeronB200Error(_lib.HB_ERR_DTYPE, "dtype %s" % dtype)
+    return code
+
+
+def _is(t, name, shape, dtype):
+    if t.shape != shape:
+        raise ValueError("%s has shape %s, the operator takes %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.dtype != dtype:
+        raise _lib.HeronB200Error(_lib.HB_ERR_DTYPE, "%s has dtype %s, the operator takes %s" % (name, t.dtype, dtype))
+
+
+def _dims(t, name, n):
+    if t.dim() != n:
+        raise ValueError("%s has %d dimensions, the operator takes %d" % (name, t.dim(), n))
+    return t.shape
+
+
+def _ptrs(*tensors):
+    """(addresses, stream) of an operator's tensors: dense, on one CUDA device, and that one current."""
+    dev = tensors[0].get_device()
+    ptrs = []
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            if not t.is_cuda:
+                raise ValueError("a tensor of shape %s must be a CUDA tensor: the kernels have no CPU path"
+                                 % (tuple(t.shape),))
+            raise ValueError("operands live on different devices: %s and %s" % (tensors[0].device, t.device))
+        if not t.is_contiguous():
+            raise ValueError("a tensor of shape %s must be contiguous" % (tuple(t.shape),))
+        ptrs.append(t.data_ptr())
+    if dev != torch.cuda.current_device():
+        _same_device(*tensors)
+    return ptrs, _raw_stream(dev)
+
+
+def _groups(offsets, groups=None):
+    n = offsets.numel() - 1
+    if offsets.dim() != 1 or n < 1 or (groups is not None and n != groups):
+        raise ValueError("offsets holds the groups' first rows and the end of the last: %s entries, got shape %s"
+                         % ("at least 2" if groups is None else groups + 1, tuple(offsets.shape)))
+    if offsets.dtype != torch.int32:
+        raise _lib.HeronB200Error(_lib.HB_ERR_DTYPE, "offsets has dtype %s, the operator takes int32" % offsets.dtype)
+    return n
+
+
+def _result(out, shape, like, out_dtype):
+    if out is None:
+        _wide_code(out_dtype or torch.float32)
+        return like.new_empty(shape, dtype=out_dtype or torch.float32)
+    _wide_code(out.dtype)
+    if out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out is %s, out_dtype is %s" % (out.dtype, out_dtype))
+    if out.shape != shape:
+        raise ValueError("out has shape %s, the operator writes %s" % (tuple(out.shape), tuple(shape)))
+    return out
+
+
+def _grouped_args(kind, first, second, offsets, out, out_dtype):
+    """(tensors in ABI order, sizes T, K, N, E and types) of one of the three grouped products."""
+    if kind == "hb_grouped_gemm_dw":
+        T, N = _dims(first, "dy", 2)
+        T2, K = _dims(second, "x", 2)
+        if T != T2:
+            raise ValueError("dy is (T,N), x is (T,K): T differs")
+        E = _groups(offsets)
+        shape = (E, N, K)
+    else:
+        T, R = _dims(first, "x" if kind == "hb_grouped_gemm" else "dy", 2)
+        E, N, K = _dims(second, "w", 3)
+        if R != (K if kind == "hb_grouped_gemm" else N):
+            raise ValueError("w is (E,N,K): its reduction axis differs from the rows' length %d" % R)
+        _groups(offsets, E)
+        shape = (T, N if kind == "hb_grouped_gemm" else K)
+    if second.dtype != first.dtype:
+        raise _lib.HeronB200Error(_lib.HB_ERR_DTYPE, "operands of %s and %s" % (first.dtype, second.dtype))
+    out = _result(out, shape, first, out_dtype)
+    return (first, second, out, offsets), (T, K, N, E, _wide_code(first.dtype), _WIDE_CODES[out.dtype])
+
+
+def _run(kind, tensors, sizes, knobs, out):
+    ptrs, stream = _ptrs(*tensors)
+    rc = getattr(_lib.load(), kind)(*ptrs, *sizes, _knobs(knobs), stream)
+    if rc:
+        _lib.check(rc, kind)
+    return out
+
+
+def _plan(kind, tensors, sizes, knobs, out):
+    h = ctypes.c_void_p()
+    name = kind.replace("hb_", "hb_plan_", 1)
+    _lib.check(getattr(_lib.load(), name)(ctypes.byref(h), *_ptrs(*tensors)[0], *sizes, _knobs(knobs)), name)
+    return Plan(h, tensors, out)
+
+
+def grouped_gemm(x, w, offsets, out=None, out_dtype=None, knobs=None):
+    """out[r] = w[e] @ x[r] for the rows r of each group e: x (T,K), w (E,N,K), out (T,N).
+
+    Group e owns rows offsets[e] .. offsets[e+1]-1 (offsets: int32 on the device, E + 1 entries; it is
+    read by the kernel, so a captured call may be replayed with other offsets).  float16 or bfloat16
+    operands, fp32 accumulation, out float32 (default), float16 or bfloat16.  K % 8 == 0.  Rows of no
+    group are left as they are in `out` (arbitrary in a fresh one)."""
+    tensors, sizes = _grouped_args("hb_grouped_gemm", x, w, offsets, out, out_dtype)
+    return _run("hb_grouped_gemm", tensors, sizes, knobs, tensors[2])
+
+
+def grouped_gemm_dx(dy, w, offsets, out=None, out_dtype=None, knobs=None):
+    """Gradient of grouped_gemm's rows: out[r] = w[e]^T @ dy[r]; dy (T,N), out (T,K).  N % 8 == K % 8 == 0."""
+    tensors, sizes = _grouped_args("hb_grouped_gemm_dx", dy, w, offsets, out, out_dtype)
+    return _run("hb_grouped_gemm_dx", tensors, sizes, knobs, tensors[2])
+
+
+def grouped_gemm_dw(dy, x, offsets, out=None, out_dtype=None, knobs=None):
+    """Gradient of grouped_gemm's weights: out[e] = sum of dy[r] x[r]^T over the rows of group e, zeros
+    for a group without rows; dy (T,N), x (T,K), out (E,N,K).  N % 8 == K % 8 == 0."""
+    tensors, sizes = _grouped_args("hb_grouped_gemm_dw", dy, x, offsets, out, out_dtype)
+    return _run("hb_grouped_gemm_dw", tensors, sizes, knobs, tensors[2])
+
+
+def plan_grouped_gemm(x, w, offsets, out=None, out_dtype=None, knobs=None):
+    tensors, sizes = _grouped_args("hb_grouped_gemm", x, w, offsets, out, out_dtype)
+    return _plan("hb_grouped_gemm", tensors, sizes, knobs, tensors[2])
+
+
+def plan_grouped_gemm_dx(dy, w, offsets, out=None, out_dtype=None, knobs=None):
+    tensors, sizes = _grouped_args("hb_grouped_gemm_dx", dy, w, offsets, out, out_dtype)
+    return _plan("hb_grouped_gemm_dx", tensors, sizes, knobs, tensors[2])
+
+
+def plan_grouped_gemm_dw(dy, x, offsets, out=None, out_dtype=None, knobs=None):
+    tensors, sizes = _grouped_args("hb_grouped_gemm_dw", dy, x, offsets, out, out_dtype)
+    return _plan("hb_grouped_gemm_dw", tensors, sizes, knobs, tensors[2])
+
+
+# ---- microscaled 4-bit floating point ----------------------------------------------------------
+def mxfp4_scale_bytes(rows, K, groups=0):
+    """Bytes of the scale array of a quantised (rows, K) matrix (include/heron_b200.h has the layout);
+    `groups`: of one whose rows are grouped by offsets."""
+    n = _lib.load().hb_mxfp4_scale_bytes(1, rows, K, groups)
+    if n == 0 and (rows > 0 or groups > 0 or K <= 0 or K % 32):
+        raise _lib.HeronB200Error(_lib.HB_ERR_SHAPE, "mxfp4_scale_bytes")
+    return n
+
+
+def _mx_shape(x, K, offsets, what):
+    """(batch, rows, groups, shape of the scales) of a matrix or batch of matrices with K elements a row."""
+    n = x.dim()
+    if n != 2 and n != 3:
+        raise ValueError("%s is (rows, K) or (batch, rows, K)" % what)
+    groups = 0
+    if offsets is not None:
+        if n != 2:
+            raise ValueError("rows grouped by offsets are a matrix (rows, K)")
+        groups = _groups(offsets)
+    rows = x.shape[-2]
+    need = mxfp4_scale_bytes(rows, K, groups)
+    return (1, rows, groups, (need,)) if n == 2 else (x.shape[0], rows, 0, (x.shape[0], need))
+
+
+def _run_mx(kind, tensors, offsets, sizes, code):
+    if offsets is None:
+        ptrs, stream = _ptrs(*tensors)
+        ptrs.append(None)
+    else:
+        ptrs, stream = _ptrs(*tensors, offsets)
+    rc = getattr(_lib.load(), kind)(*ptrs, *sizes, code, stream)
+    if rc:
+        _lib.check(rc, kind)
+
+
+def quantize_mxfp4(x, offsets=None, codes=None, scales=None):
+    """x (rows, K) or (batch, rows, K), float32, float16 or bfloat16 -> (codes, scales), uint8.
+
+    codes has x's shape with K / 2; scales is (mxfp4_scale_bytes(...),), for a batch (batch, ...).  With
+    `offsets` the rows belong to groups, as grouped_gemm_mxfp4 takes them; rows of no group are skipped.
+    K % 32 == 0."""
+    shape = x.shape
+    K = shape[-1] if shape else 0
+    code = _wide_code(x.dtype)
+    batch, rows, groups, scale_shape = _mx_shape(x, K, offsets, "x")
+    code_shape = shape[:-1] + (K // 2,)
+    if codes is None:
+        codes = x.new_empty(code_shape, dtype=torch.uint8)
+    else:
+        _is(codes, "codes", code_shape, torch.uint8)
+    if scales is None:
+        scales = x.new_empty(scale_shape, dtype=torch.uint8)
+    else:
+        _is(scales, "scales", scale_shape, torch.uint8)
+    _run_mx("hb_quantize_mxfp4", (x, codes, scales), offsets, (batch, rows, K, groups), code)
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, offsets=None, out=None, out_dtype=None):
+    """The values that quantize_mxfp4's result stands for, float32 (default), bfloat16 or float16."""
+    shape = codes.shape
+    K = 2 * shape[-1] if shape else 0
+    batch, rows, groups, scale_shape = _mx_shape(codes, K, offsets, "codes")
+    _is(codes, "codes", shape, torch.uint8)
+    _is(scales, "scales", scale_shape, torch.uint8)
+    out = _result(out, shape[:-1] + (K,), codes, out_dtype)
+    _run_mx("hb_dequantize_mxfp4", (codes, scales, out), offsets, (batch, rows, K, groups), _WIDE_CODES[out.dtype])
+    return out
+
+
+def _mx_args(a, a_scales, b, b_scales, offsets, out, out_dtype):
+    """(tensors in ABI order, sizes and type) of a product of quantised matrices."""
+    T, half = _dims(a, "a" if offsets is None else "x", 2)
+    K = 2 * half
+    if offsets is None:
+        N, half_b = _dims(b, "b", 2)
+        sizes, groups = (T, K, N), 0
+    else:
+        groups, N, half_b = _dims(b, "w", 3)
+        _groups(offsets, groups)
+        sizes = (T, K, N, groups)
+    if half != half_b:
+        raise ValueError("the operands' K differs: %d and %d code bytes a row" % (half, half_b))
+    _is(a, "the first operand", a.shape, torch.uint8)
+    _is(b, "the second operand", b.shape, torch.uint8)
+    _is(a_scales, "the first operand's scales", (mxfp4_scale_bytes(T, K, groups),), torch.uint8)
+    need = mxfp4_scale_bytes(N, K)
+    _is(b_scales, "the second operand's scales", (groups, need) if groups else (need,), torch.uint8)
+    out = _result(out, (T, N), a, out_dtype)
+    tensors = (a, a_scales, b, b_scales, out)
+    return tensors if offsets is None else tensors + (offsets,), sizes + (_WIDE_CODES[out.dtype],)
+
+
+def _needs_offsets(offsets):
+    if offsets is None:
+        raise ValueError("offsets is missing (the product without groups is gemm_mxfp4)")
+
+
+def gemm_mxfp4(a, a_scales, b, b_scales, out=None, out_dtype=None, knobs=None):
+    """out[M,N] = sum_k a[m,k] * b[n,k] over the values that two quantised matrices stand for:
+    a (M, K/2) and b (N, K/2) with the scales quantize_mxfp4 gave; out float32 (default), float16 or
+    bfloat16, fp32 accumulation."""
+    tensors, sizes = _mx_args(a, a_scales, b, b_scales, None, out, out_dtype)
+    return _run("hb_gemm_mxfp4", tensors, sizes, knobs, tensors[4])
+
+
+def grouped_gemm_mxfp4(x, x_scales, w, w_scales, offsets, out=None, out_dtype=None, knobs=None):
+    """grouped_gemm over quantised operands: x (T, K/2) quantised with the same offsets, w (E, N, K/2)
+    quantised as a batch."""
+    _needs_offsets(offsets)
+    tensors, sizes = _mx_args(x, x_scales, w, w_scales, offsets, out, out_dtype)
+    return _run("hb_grouped_gemm_mxfp4", tensors, sizes, knobs, tensors[4])
+
+
+def plan_gemm_mxfp4(a, a_scales, b, b_scales, out=None, out_dtype=None, knobs=None):
+    tensors, sizes = _mx_args(a, a_scales, b, b_scales, None, out, out_dtype)
+    return _plan("hb_gemm_mxfp4", tensors, sizes, knobs, tensors[4])
+
+
+def plan_grouped_gemm_mxfp4(x, x_scales, w, w_scales, offsets, out=None, out_dtype=None, knobs=None):
+    _needs_offsets(offsets)
+    tensors, sizes = _mx_args(x, x_scales, w, w_scales, offsets, out, out_dtype)
+    return _plan("hb_grouped_gemm_mxfp4", tensors, sizes, knobs, tensors[4])

@@ -45,7 +45,8 @@ typedef enum {
   HB_F32 = 1,
   HB_S8 = 2,
   HB_U8 = 3,
-  HB_S32 = 4
+  HB_S32 = 4,
+  HB_BF16 = 5 /* grouped and 4-bit operators only; the others answer HB_ERR_DTYPE */
 } hb_dtype;
 
 /*
@@ -299,6 +300,71 @@ int hb_conv2d_nhwc_packed_noalloc(const void* in, const void* w_packed, void* ou
                                   const hb_knobs* knobs, void* stream);
 
 /*
+ * Products grouped by expert (a mixture of experts; the reference has no counterpart, its closest
+ * operator is the batched GEMM of equal sizes, ops/cuda/batch_matmul.py).
+ *
+ * T rows of `x` belong to E groups in ascending order: group e owns rows offsets[e] ..
+ * offsets[e + 1] - 1, some of them possibly none.  `offsets` is a DEVICE array of E + 1 ints; the
+ * host never reads it, so the launch geometry does not depend on it and a captured launch may be
+ * replayed with other offsets.  Rows before offsets[0] and from offsets[E] on belong to no group:
+ * they are not read into any product and their output rows are left as they were.  Offsets are
+ * clamped to [0, T]; a group that ends before it starts is empty (rows claimed by two groups get
+ * one of the two results).
+ *
+ *   hb_grouped_gemm     out[r, n]   = sum_k x[r, k]  * w[e(r), n, k]      x (T,K), w (E,N,K), out (T,N)
+ *   hb_grouped_gemm_dx  dx[r, k]    = sum_n dy[r, n] * w[e(r), n, k]      dy (T,N), dx (T,K)
+ *   hb_grouped_gemm_dw  dw[e, n, k] = sum_{r in e} dy[r, n] * x[r, k]     dw (E,N,K), zeros for a group
+ *                                                                         without rows
+ * in: HB_F16 or HB_BF16 for both operands; out: HB_F32, HB_F16 or HB_BF16.  fp32 accumulation in a
+ * fixed order, one rounding at the end.  Dense row-major buffers; K % 8 == 0, for the gradients
+ * also N % 8 == 0; 1 <= E <= 1024; T >= 0 (T = 0: only the weight gradient is written).
+ * Knobs used: tile_n (64, 128, 192, 256: the widest tile of a group's rows; of N in dw), stages,
+ * acc_stages, cta_group (2: not dw, tile_n 128 or 256), max_ctas, silent_producer; the rest is ignored.
+ */
+int hb_grouped_gemm(const void* x, const void* w, void* out, const int* offsets, int T, int K, int N,
+                    int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream);
+int hb_grouped_gemm_dx(const void* dy, const void* w, void* dx, const int* offsets, int T, int K, int N,
+                       int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream);
+int hb_grouped_gemm_dw(const void* dy, const void* x, void* dw, const int* offsets, int T, int K, int N,
+                       int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream);
+
+/*
+ * Microscaled 4-bit floating point (MXFP4) and products of it.
+ *
+ * A matrix (rows, K), K % 32 == 0, is held as codes and scales.  32 consecutive elements of a row
+ * share the scale 2^s, s = max(floor(log2(max|x|)) - 2, -127), stored as the byte s + 127 (E8M0);
+ * an element is x * 2^-s rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to even, larger
+ * magnitudes to 6) with its sign in bit 3 (E2M1).  A block that holds an infinity or a NaN gets the
+ * scale byte 255 and elements 0, and reads back as NaN.
+ *   codes   (rows, K / 2) bytes, row-major; the even element in the low half of a byte
+ *   scales  tiles of 128 rows x 4 blocks (512 bytes), ceil(K / 128) tiles to a tile row; the scale of
+ *           row r, block b lies at ((r / 128) * ceil(K / 128) + b / 4) * 512 + (r % 32) * 16 +
+ *           (r % 128) / 32 * 4 + b % 4.  A row's bytes behind its last block are written as 0.
+ * A batch of matrices (batch, rows, K) has one such scale array per matrix, one after the other.
+ * With `groups` > 0 (and batch 1) the rows are grouped by `offsets` (device, groups + 1 ints, as in
+ * hb_grouped_gemm) and group g's first tile row is offsets[g] / 128 + g; rows of no group are skipped.
+ * hb_mxfp4_scale_bytes gives the size of the scale array (0 for sizes the operators refuse).
+ *
+ * hb_quantize_mxfp4: in HB_F16, HB_BF16 or HB_F32.  hb_dequantize_mxfp4: the values, out HB_F32,
+ * HB_BF16 (both exact) or HB_F16 (rounded; beyond its range infinite).
+ * hb_gemm_mxfp4: C[M,N] = sum_k A[m,k] * B[n,k] over the values that A (M,K) and B (N,K) stand for,
+ * fp32 accumulation, out HB_F32, HB_F16 or HB_BF16.  hb_grouped_gemm_mxfp4: hb_grouped_gemm with x
+ * quantised by groups and w (E,N,K) quantised as a batch.  Scales as written above, pad bytes
+ * included (a pad byte of 255 would turn its row into NaN).  Sizes, knobs and offsets as for
+ * hb_grouped_gemm, with K % 32 == 0 and cta_group 1.  No entry point here needs a workspace.
+ */
+size_t hb_mxfp4_scale_bytes(int batch, int rows, int K, int groups);
+int hb_quantize_mxfp4(const void* x, void* codes, void* scales, const int* offsets, int batch, int rows,
+                      int K, int groups, hb_dtype in, void* stream);
+int hb_dequantize_mxfp4(const void* codes, const void* scales, void* out, const int* offsets, int batch,
+                        int rows, int K, int groups, hb_dtype out_t, void* stream);
+int hb_gemm_mxfp4(const void* A, const void* a_scales, const void* B, const void* b_scales, void* C, int M,
+                  int K, int N, hb_dtype out_t, const hb_knobs* knobs, void* stream);
+int hb_grouped_gemm_mxfp4(const void* x, const void* x_scales, const void* w, const void* w_scales,
+                          void* out, const int* offsets, int T, int K, int N, int E, hb_dtype out_t,
+                          const hb_knobs* knobs, void* stream);
+
+/*
  * Plans.  A plan is what the reference gets back from tvm.build on an instantiated schedule
  * (tests/quick_start/dlboost/run.py:44-46) and then calls many times under time_evaluator
  * (run.py:60-62): the encoded TMA tensor maps, the resolved knobs and the launch geometry for one
@@ -337,6 +403,18 @@ int hb_plan_conv1d_ncw(hb_plan** plan, const void* in, const void* w, void* out,
 int hb_plan_conv1d_nwc_packed(hb_plan** plan, const void* in, const void* w_packed, void* out, int N,
                               int W, int CI, int CO, int KW, int stride, int pad, int dil, int sco,
                               void* scratch, size_t scratch_bytes, const hb_knobs* knobs);
+int hb_plan_grouped_gemm(hb_plan** plan, const void* x, const void* w, void* out, const int* offsets,
+                         int T, int K, int N, int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs);
+int hb_plan_grouped_gemm_dx(hb_plan** plan, const void* dy, const void* w, void* dx, const int* offsets,
+                            int T, int K, int N, int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs);
+int hb_plan_grouped_gemm_dw(hb_plan** plan, const void* dy, const void* x, void* dw, const int* offsets,
+                            int T, int K, int N, int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs);
+int hb_plan_gemm_mxfp4(hb_plan** plan, const void* A, const void* a_scales, const void* B,
+                       const void* b_scales, void* C, int M, int K, int N, hb_dtype out_t,
+                       const hb_knobs* knobs);
+int hb_plan_grouped_gemm_mxfp4(hb_plan** plan, const void* x, const void* x_scales, const void* w,
+                               const void* w_scales, void* out, const int* offsets, int T, int K, int N,
+                               int E, hb_dtype out_t, const hb_knobs* knobs);
 int hb_plan_launch(const hb_plan* plan, void* stream);
 /* The knobs after defaults were resolved, the persistent grid and the dynamic shared memory. */
 int hb_plan_knobs(const hb_plan* plan, hb_knobs* knobs, int* grid, int* smem_bytes);

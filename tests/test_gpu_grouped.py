@@ -1,0 +1,227 @@
+"""The products grouped by expert and their gradients, against a plain form in 64 bits."""
+import pytest
+import torch
+
+from grouped_util import assert_product, grouped, grouped_dw, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K(hb_lib):
+    assert torch.cuda.is_available(), "GPU tests need a B200"
+    from heron_b200 import kernels
+    assert hb_lib.hb_sm_count() > 0, "libheron_b200.so found no sm_100 device"
+    return kernels
+
+
+@pytest.fixture(autouse=True)
+def _status_clean(hb_lib):
+    yield
+    from heron_b200 import _lib
+    assert _lib.last_status() == 0, "a bounded device-side wait ran out"
+
+
+def randn(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def make(seed, counts, lead, tail, k, n, dtype):
+    """x, w, dy and offsets; rows of no group hold NaN, which must reach nothing."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    off = offsets_of(counts, lead)
+    T = off[-1] + tail
+    x, dy = randn(g, T, k, dtype=dtype), randn(g, T, n, dtype=dtype)
+    for t in (x, dy):
+        t[:lead] = torch.nan
+        t[off[-1]:] = torch.nan
+    w = randn(g, len(counts), n, k, dtype=dtype, scale=k ** -0.5)
+    return x, w, dy, off, torch.tensor(off, dtype=torch.int32, device="cuda")
+
+
+def clean(t):
+    return torch.nan_to_num(t, nan=0.0)
+
+
+COUNTS = {
+    "one_row": [1],
+    "decode": [0, 1, 0, 0, 2, 1, 0],
+    "uneven": [17, 0, 128, 1, 129, 63],
+    "all_in_one": [0, 0, 300, 0],
+    "one_group": [256],
+    "tile_edges": [16, 32, 48, 49, 64, 65],
+    "wide": [257, 511, 40],
+    "empty": [0, 0, 0],
+}
+
+
+@pytest.mark.parametrize("counts", list(COUNTS))
+@pytest.mark.parametrize("k,n", [(8, 8), (64, 128), (72, 136), (520, 264)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_forward_and_gradients(K, counts, k, n, dtype):
+    c = COUNTS[counts]
+    x, w, dy, off, offsets = make(k * 1000 + n, c, 3, 5, k, n, dtype)
+    T = x.shape[0]
+    for od in (torch.float32, dtype):
+        out = torch.full((T, n), 7.0, dtype=od, device="cuda")
+        assert K.grouped_gemm(x, w, offsets, out=out) is out
+        want, mag, own = grouped(clean(x), w, off)
+        assert_product(out[own], want[own], mag[own], k, "y")
+        assert (out[~own] == 7.0).all(), "rows of no group changed"
+        dx = torch.full((T, k), 7.0, dtype=od, device="cuda")
+        K.grouped_gemm_dx(dy, w, offsets, out=dx)
+        want, mag, own = grouped(clean(dy), w.transpose(1, 2), off)
+        assert_product(dx[own], want[own], mag[own], n, "dx")
+        assert (dx[~own] == 7.0).all(), "rows of no group changed"
+        dw = torch.full((len(c), n, k), 7.0, dtype=od, device="cuda")
+        K.grouped_gemm_dw(dy, x, offsets, out=dw)
+        want, mag = grouped_dw(clean(dy), clean(x), off, len(c))
+        assert_product(dw, want, mag, max(c), "dw")
+
+
+@pytest.mark.parametrize("n", [1, 7, 127, 1001])
+def test_forward_takes_any_output_width(K, n):
+    x, w, _, off, offsets = make(n, [5, 0, 70], 0, 0, 64, n, torch.float16)
+    for od in (torch.float32, torch.float16, torch.bfloat16):
+        want, mag, _ = grouped(x, w, off)
+        assert_product(K.grouped_gemm(x, w, offsets, out_dtype=od), want, mag, 64, str(od))
+
+
+@pytest.mark.parametrize("knobs", [dict(tile_n=64), dict(tile_n=128), dict(tile_n=192), dict(tile_n=256),
+                                   dict(tile_n=128, cta_group=2), dict(tile_n=256, cta_group=2),
+                                   dict(stages=1), dict(acc_stages=1), dict(max_ctas=2), dict(max_ctas=3, stages=2)])
+def test_knobs_do_not_change_the_product(K, knobs):
+    c = [300, 0, 1, 97, 514]
+    x, w, dy, off, offsets = make(5, c, 1, 1, 200, 328, torch.bfloat16)
+    own = grouped(clean(x), w, off)[2]
+    want, mag, _ = grouped(clean(x), w, off)
+    assert_product(K.grouped_gemm(x, w, offsets, knobs=knobs)[own], want[own], mag[own], 200, "y")
+    want, mag, _ = grouped(clean(dy), w.transpose(1, 2), off)
+    assert_product(K.grouped_gemm_dx(dy, w, offsets, knobs=knobs)[own], want[own], mag[own], 328, "dx")
+    if knobs.get("cta_group") != 2:
+        want, mag = grouped_dw(clean(dy), clean(x), off, len(c))
+        assert_product(K.grouped_gemm_dw(dy, x, offsets, knobs=knobs), want, mag, 514, "dw")
+
+
+def test_an_infinity_stays_in_its_group(K):
+    x, w, dy, off, offsets = make(3, [5, 9, 20], 0, 0, 64, 64, torch.float16)
+    x[6], dy[6] = torch.inf, torch.nan
+    y = K.grouped_gemm(x, w, offsets)
+    assert torch.isfinite(y[:6]).all() and torch.isfinite(y[7:]).all() and not torch.isfinite(y[6]).any()
+    dw = K.grouped_gemm_dw(dy, x, offsets)
+    assert torch.isfinite(dw[0]).all() and torch.isfinite(dw[2]).all() and torch.isnan(dw[1]).all()
+
+
+def test_many_groups(K):
+    g = torch.Generator().manual_seed(1)
+    c = torch.randint(0, 3, (1024,), generator=g).tolist()
+    x, w, dy, off, offsets = make(9, c, 0, 0, 64, 72, torch.bfloat16)
+    want, mag, _ = grouped(x, w, off)
+    assert_product(K.grouped_gemm(x, w, offsets), want, mag, 64, "y")
+    want, mag = grouped_dw(dy, x, off, 1024)
+    assert_product(K.grouped_gemm_dw(dy, x, offsets), want, mag, 2, "dw")
+
+
+def test_no_rows(K):
+    w = torch.ones(3, 16, 8, dtype=torch.float16, device="cuda")
+    offsets = torch.zeros(4, dtype=torch.int32, device="cuda")
+    assert K.grouped_gemm(w.new_empty(0, 8), w, offsets).shape == (0, 16)
+    assert K.grouped_gemm_dx(w.new_empty(0, 16), w, offsets).shape == (0, 8)
+    dw = torch.full((3, 16, 8), 7.0, device="cuda")
+    K.grouped_gemm_dw(w.new_empty(0, 16), w.new_empty(0, 8), offsets, out=dw)
+    assert (dw == 0).all()
+    plan = K.plan_grouped_gemm_dw(w.new_empty(0, 16), w.new_empty(0, 8), offsets, out=dw.fill_(7.0))
+    plan.launch()
+    assert (dw == 0).all()
+
+
+@pytest.mark.parametrize("off", [[-5, 4, 8], [0, 4, 1000], [6, 2, 8], [8, 8, 8], [0, 2 ** 31 - 1, 8]])
+def test_offsets_are_clamped(K, off):
+    """Offsets outside the rows or out of order: rows that one group owns are right, the others untouched."""
+    from grouped_util import clamped
+    x, w, dy, _, _ = make(4, [8, 0], 0, 0, 64, 64, torch.float16)
+    offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+    owners = torch.zeros(8, dtype=torch.int64)
+    for s, t in clamped(off, 8):
+        owners[s:t] += 1
+    once = (owners == 1).cuda()
+    out = torch.full((8, 64), 7.0, device="cuda")
+    K.grouped_gemm(x, w, offsets, out=out)
+    want, mag, _ = grouped(x, w, off)
+    assert_product(out[once], want[once], mag[once], 64)
+    assert (out[(owners == 0).cuda()] == 7.0).all()
+    want, mag = grouped_dw(dy, x, off, 2)
+    assert_product(K.grouped_gemm_dw(dy, x, offsets), want, mag, 8)
+
+
+def test_graph_replay_with_other_offsets_and_streams(K):
+    x, w, dy, off, offsets = make(6, [40, 3, 90], 0, 0, 128, 192, torch.bfloat16)
+    out = torch.empty(133, 192, device="cuda")
+    dw = torch.empty(3, 192, 128, device="cuda")
+    plan = K.plan_grouped_gemm(x, w, offsets, out=out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            plan.launch()
+            K.grouped_gemm_dw(dy, x, offsets, out=dw)
+    torch.cuda.current_stream().wait_stream(side)
+    for other in ([0, 40, 43, 133], [0, 0, 133, 133], [0, 65, 66, 133]):
+        offsets.copy_(torch.tensor(other, dtype=torch.int32))
+        out.fill_(7.0)
+        dw.fill_(7.0)
+        graph.replay()
+        want, mag, _ = grouped(x, w, other)
+        assert_product(out, want, mag, 128)
+        want, mag = grouped_dw(dy, x, other, 3)
+        assert_product(dw, want, mag, 133)
+    # two streams at once
+    res = []
+    for _ in range(2):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            res.append([K.grouped_gemm(x, w, offsets) for _ in range(4)])
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for r in res:
+        for y in r:
+            assert torch.equal(y, res[0][0])
+
+
+def test_gradients_against_differences(K):
+    """The directional derivative of sum(c * y) by central differences of the forward operator.  y is linear in
+    x and in w, so the difference quotient has no truncation error, only that of two forward passes."""
+    x, w, dy, off, offsets = make(8, [20, 0, 44], 0, 0, 64, 128, torch.float16)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    # a direction and a step that fp16 holds exactly: multiples of 2^-6 on values rounded to 2^-6
+    x = (x * 64).round() / 64
+    w = (w * 64).round() / 64
+    vx = torch.randint(-2, 3, x.shape, generator=g, device="cuda").half() / 64
+    vw = torch.randint(-2, 3, w.shape, generator=g, device="cuda").half() / 64
+    dx, dw = K.grouped_gemm_dx(dy, w, offsets), K.grouped_gemm_dw(dy, x, offsets)
+    up, down = (K.grouped_gemm(x + s * vx, w, offsets).double() for s in (1, -1))
+    mag = grouped(x.abs() + vx.abs(), w.abs(), off)[1]
+    tol = 64 * 2.0 ** -23 * (2 * mag * dy.double().abs()).sum() + \
+        128 * 2.0 ** -23 * (grouped(dy, w.transpose(1, 2), off)[1] * vx.double().abs()).sum() * 2
+    assert abs(((up - down) * dy.double()).sum() - 2 * (dx.double() * vx.double()).sum()) <= tol
+    up, down = (K.grouped_gemm(x, w + s * vw, offsets).double() for s in (1, -1))
+    mag = grouped(x.abs(), w.abs() + vw.abs(), off)[1]
+    tol = 64 * 2.0 ** -23 * (2 * mag * dy.double().abs()).sum() + \
+        44 * 2.0 ** -23 * (grouped_dw(dy, x, off, 3)[1] * vw.double().abs()).sum() * 2
+    assert abs(((up - down) * dy.double()).sum() - 2 * (dw.double() * vw.double()).sum()) <= tol
+
+
+def test_a_silent_producer_ends_in_a_status(K):
+    """The bounded waits: nothing is loaded, the launch ends by itself and reports it."""
+    from heron_b200 import _lib
+    x, w, dy, off, offsets = make(6, [40, 3, 90], 0, 0, 128, 192, torch.bfloat16)
+    for fn, args in ((K.grouped_gemm, (x, w)), (K.grouped_gemm_dx, (dy, w)), (K.grouped_gemm_dw, (dy, x))):
+        fn(*args, offsets, knobs=dict(silent_producer=1))
+        assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
+    fn = K.grouped_gemm
+    fn(x, w, offsets, knobs=dict(silent_producer=1, cta_group=2, tile_n=128))
+    assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
+    want, mag, _ = grouped(x, w, off)
+    assert_product(K.grouped_gemm(x, w, offsets), want, mag, 128)
