@@ -42,7 +42,8 @@ namespace hb {
 enum { kFwd = 0, kDx = 1, kDw = 2, kMx = 3 };
 
 constexpr int kMaxGroups = 1024;
-constexpr int kGroupThreads = 32 * 7;  // A producer, MMA, four epilogue warps, B producer
+// A producer, MMA, four epilogue warps, B producer; kMx: the copies of the scales
+__host__ __device__ constexpr int group_threads(int mode) { return mode == kMx ? 256 : 224; }
 constexpr int kSpan = 128;             // bytes of the reduction axis in a ring stage (TMA swizzle span)
 constexpr int kAtomBytes = 512;        // scales of 128 rows x 128 elements
 
@@ -161,9 +162,10 @@ __device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, i
 struct GroupBars {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
+  uint64_t sf_full[kMaxStages];
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
-  uint64_t drain;
+  uint64_t drain, sf_drain;
   uint32_t tmem_base;
   int abort_flag;
   int total;
@@ -178,7 +180,7 @@ __host__ __device__ __forceinline__ int group_stage_bytes(int BN) {
 }
 
 template <int MODE, int CG>
-__global__ void __launch_bounds__(kGroupThreads, 1)
+__global__ void __launch_bounds__(group_threads(MODE), 1)
 hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmB16, const GroupParams p) {
   constexpr bool A_MN = MODE == kDx || MODE == kDw;
@@ -208,12 +210,14 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
+      mbar_init(smem_u32(&bars->sf_full[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&bars->tmem_full[a]), 1);
       mbar_init(smem_u32(&bars->tmem_empty[a]), 4 * CG);
     }
     mbar_init(smem_u32(&bars->drain), 1);
+    mbar_init(smem_u32(&bars->sf_drain), 1);
     bars->abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmA);
@@ -339,6 +343,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     constexpr uint32_t a_lo_fixed = (A_MN ? chunk16 : 1u) << 16, b_lo_fixed = (B_MN ? chunk16 : 1u) << 16;
     constexpr uint32_t a_step = A_MN ? 16u * kSpan >> 4 : 2u, b_step = B_MN ? 16u * kSpan >> 4 : 2u;
     const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
+    const uint32_t sf_full0 = smem_u32(&bars->sf_full[0]);
     const uint32_t sf_cols = static_cast<uint32_t>(8 * (1 + sf_rows));  // TMEM columns of a stage's scales
     const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
     int at = 0;
@@ -351,9 +356,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * p.BN);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tl.nmma >> 3) << 17);
       uint32_t accum = 0u;
-      const int nb_sf = MODE == kMx ? sf_b_rows(tl) : 0;
       for (int kb = 0; kb < tl.blocks; ++kb) {
         ok = all_lanes(mbar_wait(full0 + 8u * stage, phase, wctx));
+        if (MODE == kMx && ok) ok = mbar_wait(sf_full0 + 8u * stage, phase, wctx);
         if (!ok) break;
         tc_fence_after();
         const uint32_t stA = sA + stage * a_bytes, stB = sB + stage * b_bytes;
@@ -379,19 +384,8 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           const uint32_t a_lo = ((stA >> 4) & 0x3FFFu) | a_lo_fixed, b_lo = ((stB >> 4) & 0x3FFFu) | b_lo_fixed;
           uint32_t ta = 0, tb = 0;
           if constexpr (MODE == kMx) {
-            // scales into TMEM.  A stage has its own columns: they are written again only after the
-            // MMAs that read them have freed the stage.  Columns: A's two tiles of 128 elements, then
-            // per tile of 128 elements B's tile rows side by side (column j holds rows 32 j ...).
             ta = sf_tmem + stage * sf_cols;
-            tb = ta + 8u;
-            const uint32_t sf = sSF + stage * sf_bytes;
-            const int tiles_k = min(2, (p.R - kb * kElems + 127) / 128);
-            for (int ka = 0; ka < tiles_k; ++ka) {
-              tmem_cp_scales(ta + 4u * ka, sf + ka * kAtomBytes);
-              for (int i = 0; i < nb_sf; ++i)
-                tmem_cp_scales(tb + static_cast<uint32_t>(ka * 4 * sf_rows + 4 * i), sf + ((1 + i) * 2 + ka) * kAtomBytes);
-            }
-            tb += static_cast<uint32_t>((tl.c0 & 127) >> 5);
+            tb = ta + 8u + static_cast<uint32_t>((tl.c0 & 127) >> 5);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -425,6 +419,46 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   };
 
+  // kMx: the scales of a stage from shared memory to TMEM, by a thread of its own (see kMx above).  A
+  // stage has its own columns: they are written again only after the MMAs that read them have freed the
+  // stage.  Columns: A's two tiles of 128 elements, then per tile of 128 elements B's tile rows side by
+  // side (column j holds rows 32 j ...).
+  auto copy_scales = [&]() {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t sf_cols = static_cast<uint32_t>(8 * (1 + sf_rows));
+    const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
+    int at = 0;
+    GroupTile tl;
+    for (int t = first_tile; ok && group_tile<MODE, CG>(p, groups, at, t, total, tl); t += tile_step) {
+      const int nb_sf = sf_b_rows(tl);
+      for (int kb = 0; kb < tl.blocks; ++kb) {
+        if (!mbar_wait(smem_u32(&bars->full[stage]), phase, wctx)) {
+          ok = false;
+          break;
+        }
+        const uint32_t ta = sf_tmem + stage * sf_cols, tb = ta + 8u;
+        const uint32_t sf = sSF + stage * sf_bytes;
+        const int tiles_k = min(2, (p.R - kb * kElems + 127) / 128);
+        for (int ka = 0; ka < tiles_k; ++ka) {
+          tmem_cp_scales(ta + 4u * ka, sf + ka * kAtomBytes);
+          for (int i = 0; i < nb_sf; ++i)
+            tmem_cp_scales(tb + static_cast<uint32_t>(ka * 4 * sf_rows + 4 * i), sf + ((1 + i) * 2 + ka) * kAtomBytes);
+        }
+        umma_commit(smem_u32(&bars->sf_full[stage]));
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok) {
+      umma_commit(smem_u32(&bars->sf_drain));
+      mbar_wait_drain(smem_u32(&bars->sf_drain), 0u);
+    }
+  };
+
   if (warp == 0) {
     if (elect_one()) produce(1);
     __syncwarp();
@@ -440,6 +474,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     __syncwarp();
   } else if (warp == 6) {
     if (elect_one()) produce(2);
+    __syncwarp();
+  } else if (MODE == kMx && warp == 7) {
+    if (elect_one()) copy_scales();
     __syncwarp();
   } else {
     const int q = warp & 3;

@@ -188,7 +188,7 @@ int launch_group(const hb_plan* plan, cudaStream_t stream) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(plan->grid);
-  cfg.blockDim = dim3(hb::kGroupThreads);
+  cfg.blockDim = dim3(hb::group_threads(MODE));
   cfg.dynamicSmemBytes = plan->smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -245,14 +245,14 @@ int run_mx(bool back, const void* values, const void* codes, const void* scales,
   p.offsets = offsets;
   p.batch = batch; p.rows = rows; p.K = K; p.groups = groups;
   p.matrix_scales = static_cast<long long>(mx_scale_bytes(1, rows, K, groups));
-  const long long units = static_cast<long long>(batch) * rows * ((K + 127) / 128);
-  const long long blocks = (units + hb::kMxThreads / 16 - 1) / (hb::kMxThreads / 16);
-  const long long cap = static_cast<long long>(d.sm_count) * 8;
+  // 16 blocks of eight rows to a tile row of scales
+  const long long row_blocks = 16LL * batch * (groups > 0 ? rows / 128 + groups : (rows + 127LL) / 128);
+  const int segments = (K - 1) / hb::kMxSegment + 1;
+  if (segments > 65535 || row_blocks > 0x7fffffffLL) return HB_ERR_SHAPE;
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks < cap ? blocks : cap));
+  cfg.gridDim = dim3(static_cast<unsigned>(row_blocks), segments);
   cfg.blockDim = dim3(hb::kMxThreads);
-  cfg.dynamicSmemBytes = groups > 0 ? (groups + 1) * sizeof(int) : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

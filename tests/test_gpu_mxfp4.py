@@ -92,6 +92,16 @@ def test_quantise_by_groups(K, counts, lead, tail):
     check_quantised(K, x, torch.tensor(off, dtype=torch.int32, device="cuda"), off)
 
 
+@pytest.mark.parametrize("E", [31, 33, 64, 100, 1024])
+def test_quantise_by_many_groups(K, E):
+    g = torch.Generator().manual_seed(E)
+    counts = (torch.randint(0, 5, (E,), generator=g) * (torch.rand(E, generator=g) < 0.6)).tolist()
+    counts[E // 2] = 150
+    off = offsets_of(counts, 2)
+    x = randn(E, off[-1] + 1, 64, dtype=torch.bfloat16)
+    check_quantised(K, x, torch.tensor(off, dtype=torch.int32, device="cuda"), off)
+
+
 def test_quantise_a_batch(K):
     x = randn(3, 3, 130, 96, dtype=torch.float16)
     codes, scales = K.quantize_mxfp4(x)
