@@ -13,6 +13,9 @@ CSRC = os.path.join(HERE, "csrc")
 TARGET = os.path.join(HERE, "libheron_b200.so")
 SOURCES = [os.path.join(CSRC, "hb_api.cu")]
 HEADER = os.path.join(HERE, os.pardir, "include", "heron_b200.h")
+# the C++ front end of the grouped and 4-bit operators (a CPython extension next to the library)
+FRONT = os.path.join(HERE, "_front.so")
+FRONT_SOURCE = os.path.join(CSRC, "hb_front.cpp")
 
 
 def deps():
@@ -40,24 +43,52 @@ def is_stale():
     return any(os.path.exists(d) and os.path.getmtime(d) > t for d in deps())
 
 
+def _run(cmd, target, verbose):
+    """Runs a compiler command with its output beside the target and moved into place, so that a
+    reader never sees a half-written file."""
+    tmp = target + ".tmp.%d" % os.getpid()
+    cmd = cmd + ["-o", tmp]
+    if verbose:
+        print(" ".join(cmd))
+    try:
+        subprocess.check_call(cmd)
+        os.replace(tmp, target)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+
+
+def build_front(force=False, verbose=False):
+    """heron_b200/_front.so, linked against the library beside it and torch's own libraries."""
+    sources = (FRONT_SOURCE, HEADER, os.path.abspath(__file__))
+    if not force and os.path.exists(FRONT) and all(os.path.getmtime(s) <= os.path.getmtime(FRONT) for s in sources):
+        return FRONT
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    inc = cpp_extension.include_paths() + ["/usr/local/cuda/include", sysconfig.get_paths()["include"]]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+         + [f for i in inc for f in ("-isystem", i)] + [FRONT_SOURCE, "-L" + HERE, "-l:libheron_b200.so", "-L" + lib,
+         "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], FRONT, verbose)
+    return FRONT
+
+
 def build(force=False, verbose=False, extra_flags=()):
+    """Builds what is out of date and returns the library's path."""
+    build_library(force, verbose, extra_flags)
+    build_front(force, verbose)
+    return TARGET
+
+
+def build_library(force=False, verbose=False, extra_flags=()):
     """Diagnostic probe modes (knob ``probe``) are compiled in only when HB_PROBES=1 is set in the
     environment; the shipped library has none of their branches."""
     if not force and not is_stale():
         return TARGET
     if os.environ.get("HB_PROBES") == "1":
         extra_flags = list(extra_flags) + ["-DHB_PROBES"]
-    # (built beside the target and moved into place, so a reader never sees a half-written library)
-    tmp = TARGET + ".tmp.%d" % os.getpid()
-    cmd = [nvcc()] + NVCC_FLAGS + list(extra_flags) + ["-o", tmp] + SOURCES
-    if verbose:
-        print(" ".join(cmd))
-    try:
-        subprocess.check_call(cmd)
-        os.replace(tmp, TARGET)
-    finally:
-        if os.path.exists(tmp):
-            os.remove(tmp)
+    _run([nvcc()] + NVCC_FLAGS + list(extra_flags) + SOURCES, TARGET, verbose)
     return TARGET
 
 

@@ -25,8 +25,8 @@
 //
 // Operand layouts, the ring of TMA stages, the roles of the warps and the bounded waits are those of
 // hb_umma_kernel (hb_kernel.cuh).  In kDw a group's last block of 64 rows usually reaches into the
-// next group: the MMA warp writes zeros over those rows of both operands (another group's infinity
-// times zero would be NaN) up to the next multiple of 16 and issues no MMA beyond it.
+// next group: a warp writes zeros over those rows of both operands (another group's infinity times zero
+// would be NaN) up to the next multiple of 16, and no MMA is issued beyond it.
 //
 // Tiles are listed on the device: every CTA reads the offsets, keeps the groups that have rows (all
 // of them in kDw) with a running count of tiles in shared memory, and walks tiles blockIdx.x,
@@ -42,8 +42,12 @@ namespace hb {
 enum { kFwd = 0, kDx = 1, kDw = 2, kMx = 3 };
 
 constexpr int kMaxGroups = 1024;
-// A producer, MMA, four epilogue warps, B producer; kMx: the copies of the scales
-__host__ __device__ constexpr int group_threads(int mode) { return mode == kMx ? 256 : 224; }
+constexpr int kSortedGroups = 224;  // a thread each
+// A producer, MMA, eight epilogue warps, B producer; kDw: the zeros behind a group; kMx: the copies of the
+// scales and their producer
+constexpr int kGroupEpi = 8;
+__host__ __device__ constexpr int group_threads(int mode) { return 32 * (3 + kGroupEpi + (mode == kMx ? 2 : (mode == kDw ? 1 : 0))); }
+constexpr int kGroupStage = 2048;      // epilogue staging of a warp: 32 columns x 32 16-bit values
 constexpr int kSpan = 128;             // bytes of the reduction axis in a ring stage (TMA swizzle span)
 constexpr int kAtomBytes = 512;        // scales of 128 rows x 128 elements
 
@@ -56,6 +60,8 @@ struct GroupParams {
   int BN;               // widest tile, multiple of 32 (64 in kDw and kMx)
   int stages, acc_stages, tmem_cols, tiles_m;
   int out_type;         // 0: fp32, 1: fp16, 2: bf16
+  int wide_rows;        // 16-bit output whose rows are multiples of 16 bytes
+  int sorted;           // more tiles than CTAs: groups in order of their tiles' cost, see group_list
   uint32_t idesc;       // without the N field
   void* out;
   long long ldc;        // elements between consecutive output rows
@@ -125,16 +131,42 @@ __device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, i
       s = min(max(p.offsets[e], 0), p.T);
       t = min(max(p.offsets[e + 1], s), p.T);
     }
+    g[e].e = e;
     g[e].start = s;
     g[e].n = t - s;
   }
   __syncthreads();
+  if (p.sorted) {
+    // Groups by falling cost of a tile (rows in kDw, the tile's width otherwise): the tiles dealt out last
+    // are then the small ones, and every second round deals them in reverse.
+    const int i = threadIdx.x;  // (host: sorted only with E <= kSortedGroups threads)
+    GroupEntry mine{0, 0, 0, 0};
+    if (i < p.E) {
+      mine = g[i];
+      const int n = mine.n;
+      mine.end_tile = MODE == kDw ? n : (n == 0 ? 0 : min(n, group_width<MODE, CG>(n, (n + p.BN - 1) / p.BN, p.BN)));
+      g[i].end_tile = mine.end_tile;
+    }
+    __syncthreads();
+    int rank = 0;
+    if (i < p.E) {
+#pragma unroll 8
+      for (int j = 0; j < p.E; ++j) {
+        const int d = g[j].end_tile;
+        rank += d > mine.end_tile || (d == mine.end_tile && j < i);
+      }
+    }
+    __syncthreads();
+    if (i < p.E) g[rank] = mine;
+    __syncthreads();
+  }
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int kept = 0, sum = 0;
     for (int base = 0; base < p.E; base += 32) {
       const int e = base + lane;
-      const int start = e < p.E ? g[e].start : 0, n = e < p.E ? g[e].n : 0;
+      const GroupEntry in = e < p.E ? g[e] : GroupEntry{0, 0, 0, 0};
+      const int n = in.n;
       const int cols = MODE == kDw ? (e < p.E ? p.C : 0) : n;
       int tiles = (cols + p.BN - 1) / p.BN * p.tiles_m;
       const uint32_t has = __ballot_sync(0xffffffffu, tiles > 0);
@@ -147,7 +179,7 @@ __device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, i
       // (every lane holds its group in registers: the entries written below are at or before these)
       if (tiles > 0) {
         const int slot = kept + __popc(has & ((1u << lane) - 1u));
-        g[slot] = GroupEntry{e, start, n, sum + incl};
+        g[slot] = GroupEntry{in.e, in.start, n, sum + incl};
       }
       __syncwarp();
       kept += __popc(has);
@@ -162,7 +194,7 @@ __device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, i
 struct GroupBars {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
-  uint64_t sf_full[kMaxStages];
+  uint64_t sf_full[kMaxStages];  // kMx: the stage's scales are in TMEM; kDw: its edge is zero
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
   uint64_t drain, sf_drain;
@@ -179,10 +211,21 @@ __host__ __device__ __forceinline__ int group_stage_bytes(int BN) {
   return (kTileM + BN / CG) * kSpan + (MODE == kMx ? (1 + group_sf_rows(BN)) * 2 * kAtomBytes : 0);
 }
 
+// Two accumulators rounded to the 16-bit output type (one rounding, to nearest even).
+__device__ __forceinline__ uint32_t pack16(int out_type, uint32_t a, uint32_t b) {
+  if (out_type == 1) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(a), __uint_as_float(b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <int MODE, int CG>
 __global__ void __launch_bounds__(group_threads(MODE), 1)
 hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                const __grid_constant__ CUtensorMap tmB16, const GroupParams p) {
+                const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ CUtensorMap tmBw,
+                const GroupParams p) {
   constexpr bool A_MN = MODE == kDx || MODE == kDw;
   constexpr bool B_MN = MODE == kDw;
   constexpr int kElems = MODE == kMx ? 256 : 64;
@@ -198,7 +241,8 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const uint32_t sA = smem_base;
   const uint32_t sB = sA + p.stages * a_bytes;
   const uint32_t sSF = sB + p.stages * b_bytes;
-  uint8_t* after = smem + (sSF - smem_base) + p.stages * sf_bytes;
+  const uint32_t sEpi = sSF + p.stages * sf_bytes;
+  uint8_t* after = smem + (sEpi - smem_base) + kGroupEpi * kGroupStage;
   GroupBars* bars = reinterpret_cast<GroupBars*>(after);
   GroupEntry* groups = reinterpret_cast<GroupEntry*>(after + ((sizeof(GroupBars) + 15) & ~15));
   volatile int* abort_flag = &bars->abort_flag;
@@ -209,12 +253,12 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
-      mbar_init(smem_u32(&bars->empty[s]), 1);
+      mbar_init(smem_u32(&bars->empty[s]), MODE == kDw ? 2 : 1);
       mbar_init(smem_u32(&bars->sf_full[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&bars->tmem_full[a]), 1);
-      mbar_init(smem_u32(&bars->tmem_empty[a]), 4 * CG);
+      mbar_init(smem_u32(&bars->tmem_empty[a]), kGroupEpi * CG);
     }
     mbar_init(smem_u32(&bars->drain), 1);
     mbar_init(smem_u32(&bars->sf_drain), 1);
@@ -235,16 +279,24 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const int first_tile = blockIdx.x / CG;
   const int tile_step = gridDim.x / CG;
 
-  // B rows (K-major) or columns (MN-major) of a tile that this CTA stages, and how they are fetched
-  // (boxes of 16 rows for narrow tiles, of 64 otherwise)
+  // the i-th tile of this CTA (pair)
+  auto tile_of = [&](int i) {
+    return i * tile_step + (p.sorted && (i & 1) ? tile_step - 1 - first_tile : first_tile);
+  };
+
+  // B rows (K-major) or columns (MN-major) of a tile that this CTA stages, and how they are fetched: boxes
+  // of 16 rows for narrow tiles, one box of the widest tile where that reads at most a third too much (a
+  // load costs its issuing thread 85 cycles: with boxes of 64 throughout, that thread bounded the 4-bit
+  // product of 192-row tiles), of 64 otherwise
   auto b_boxes = [&](int nmma, int& box) {
     const int mine = nmma / CG;
-    box = (!B_MN && mine <= 48) ? 16 : 64;
+    if (B_MN) box = 64;
+    else box = mine <= 48 ? 16 : (4 * mine >= 3 * (p.BN / CG) ? p.BN / CG : 64);
     return (mine + box - 1) / box;
   };
   auto sf_b_rows = [&](const GroupTile& tl) { return ((tl.c0 & 127) + tl.nmma + 127) >> 7; };
 
-  // part bit 0: A (and the barrier's byte count); bit 1: B
+  // part bit 0: A (and the barrier's byte count); bit 1: B; bit 2: kMx's scales
   auto produce = [&](int part) {
     int stage = 0;
     uint32_t phase = 0;
@@ -253,8 +305,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     int at = 0;
     GroupTile tl;
     const int kt = MODE == kMx ? (p.R + 127) / 128 : 0;  // scale tiles along the reduction
-    for (int t = first_tile; ok && !p.silent_producer && group_tile<MODE, CG>(p, groups, at, t, total, tl);
-         t += tile_step) {
+    for (int i = 0; ok && !p.silent_producer && group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
       int box;
       const int boxes = b_boxes(tl.nmma, box);
       const uint32_t tx_ab = static_cast<uint32_t>(a_bytes + boxes * box * kSpan) * CG;
@@ -288,19 +339,26 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             tma_load_3d_cg<CG>(dA, &tmA, full, m0, row, z);
             tma_load_3d_cg<CG>(dA + a_bytes / 2, &tmA, full, m0 + 64, row, z);
           }
-          if (MODE == kMx) bulk_load(dSF, sfa + static_cast<long long>(kb) * 2 * kAtomBytes, sf_tile, full);
         }
         if (part & 2) {
-          const CUtensorMap* tb = box == 16 ? &tmB16 : &tmB;
-          for (int i = 0; i < boxes; ++i) {
-            if (B_MN)
-              tma_load_3d_cg<CG>(dB + i * 64 * kSpan, tb, full, mine0 + i * 64, tl.start + red, 0);
-            else
-              tma_load_3d_cg<CG>(dB + i * box * kSpan, tb, full, red, tl.start + mine0 + i * box, 0);
+          if (B_MN) {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d_cg<CG>(dB + b * 64 * kSpan, &tmB, full, mine0 + b * 64, tl.start + red, 0);
+          } else if (boxes == 1 && box > 64) {
+            tma_load_3d_cg<CG>(dB, &tmBw, full, red, tl.start + mine0, 0);
+          } else if (box == 16) {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d_cg<CG>(dB + b * 16 * kSpan, &tmB16, full, red, tl.start + mine0 + b * 16, 0);
+          } else {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d_cg<CG>(dB + b * 64 * kSpan, &tmB, full, red, tl.start + mine0 + b * 64, 0);
           }
-          for (int i = 0; i < nb_sf; ++i)
-            bulk_load(dSF + (1 + i) * 2 * kAtomBytes,
-                      sfb + (static_cast<long long>(i) * kt + 2 * kb) * kAtomBytes, sf_tile, full);
+        }
+        if (MODE == kMx && (part & 4)) {
+          bulk_load(dSF, sfa + static_cast<long long>(kb) * 2 * kAtomBytes, sf_tile, full);
+          for (int b = 0; b < nb_sf; ++b)
+            bulk_load(dSF + (1 + b) * 2 * kAtomBytes, sfb + (static_cast<long long>(b) * kt + 2 * kb) * kAtomBytes,
+                      sf_tile, full);
         }
         ++issued;
         if (++stage == p.stages) {
@@ -327,15 +385,14 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   };
 
-  // The MMA role.  One elected lane issues; in kDw the whole warp walks along, to write the zeros
-  // behind a group's last row.
-  auto multiply = [&](bool issue) {
+  // The MMA role, one elected lane.
+  auto multiply = [&]() {
     int stage = 0;
     uint32_t phase = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    auto all_lanes = [](bool v) { return MODE == kDw ? __all_sync(0xffffffffu, v) != 0 : v; };
+    uint32_t edges = 0;  // kDw: parity of each stage's next wait for its edge's zeros
     constexpr uint32_t layout_type = 2u;  // 128-byte swizzle
     constexpr uint64_t desc_hi = static_cast<uint64_t>(((8u * kSpan) >> 4) | (1u << 14) | (layout_type << 29)) << 32;
     // MN-major: 64 x 64 chunks of 8 KB, 16 reduction rows (2 KB) per MMA; K-major: 32 bytes per MMA
@@ -348,16 +405,16 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
     int at = 0;
     GroupTile tl;
-    for (int t = first_tile; ok && group_tile<MODE, CG>(p, groups, at, t, total, tl); t += tile_step) {
+    for (int i = 0; ok && group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
       if (MODE == kDw && tl.blocks == 0) continue;  // (the epilogue writes zeros without an accumulator)
-      ok = all_lanes(mbar_wait(smem_u32(&bars->tmem_empty[acc]), acc_phase ^ 1u, wctx));
+      ok = mbar_wait(smem_u32(&bars->tmem_empty[acc]), acc_phase ^ 1u, wctx);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * p.BN);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tl.nmma >> 3) << 17);
       uint32_t accum = 0u;
       for (int kb = 0; kb < tl.blocks; ++kb) {
-        ok = all_lanes(mbar_wait(full0 + 8u * stage, phase, wctx));
+        ok = mbar_wait(full0 + 8u * stage, phase, wctx);
         if (MODE == kMx && ok) ok = mbar_wait(sf_full0 + 8u * stage, phase, wctx);
         if (!ok) break;
         tc_fence_after();
@@ -366,21 +423,19 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         int steps = 4;
         if (MODE == kMx) steps = min(4, (p.R - kb * kElems + 63) / 64);
         if (MODE == kDw) {
-          const int valid = min(64, tl.n - kb * 64);
+          const int valid = tl.n - kb * 64;
           if (valid < 64) {
             steps = (valid + 15) / 16;
-            const int chunks = 2 + (tl.nmma + 63) / 64;
-            const int vecs = (steps * 16 - valid) * 8;  // 16-byte vectors of a 64-column chunk
-            for (int c = 0; c < chunks; ++c) {
-              const uint32_t base = (c < 2 ? stA + c * 64 * kSpan : stB + (c - 2) * 64 * kSpan) + valid * kSpan;
-              for (int v = lane; v < vecs; v += 32)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + v * 16), "r"(0) : "memory");
+            if (valid & 15) {  // (the rows behind the group's last one are zero when this barrier says so)
+              if (!mbar_wait(sf_full0 + 8u * stage, (edges >> stage) & 1u, wctx)) {
+                ok = false;
+                break;
+              }
+              edges ^= 1u << stage;
             }
-            fence_proxy_async_smem();
-            __syncwarp();
           }
         }
-        if (issue) {
+        {
           const uint32_t a_lo = ((stA >> 4) & 0x3FFFu) | a_lo_fixed, b_lo = ((stB >> 4) & 0x3FFFu) | b_lo_fixed;
           uint32_t ta = 0, tb = 0;
           if constexpr (MODE == kMx) {
@@ -407,13 +462,13 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
       }
       if (!ok) break;
-      if (issue) umma_commit_cg<CG>(smem_u32(&bars->tmem_full[acc]));
+      umma_commit_cg<CG>(smem_u32(&bars->tmem_full[acc]));
       if (++acc == p.acc_stages) {
         acc = 0;
         acc_phase ^= 1u;
       }
     }
-    if (!ok && issue) {
+    if (!ok) {
       umma_commit_local<CG>(smem_u32(&bars->drain));
       mbar_wait_drain(smem_u32(&bars->drain), 0u);
     }
@@ -431,7 +486,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
     int at = 0;
     GroupTile tl;
-    for (int t = first_tile; ok && group_tile<MODE, CG>(p, groups, at, t, total, tl); t += tile_step) {
+    for (int i = 0; ok && group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
       const int nb_sf = sf_b_rows(tl);
       for (int kb = 0; kb < tl.blocks; ++kb) {
         if (!mbar_wait(smem_u32(&bars->full[stage]), phase, wctx)) {
@@ -459,32 +514,90 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   };
 
+  // kDw: the rows behind a group's last one in its last block, up to the next multiple of 16, set to zero in
+  // both operands as soon as the block has landed.  A warp of its own: done by the MMA warp it held up
+  // every tile by some 2500 cycles.
+  auto clear_edges = [&]() {
+    int stage = 0, at = 0;
+    uint32_t phase = 0;
+    GroupTile tl;
+    for (int i = 0; group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
+      const int valid = tl.n & 15 ? tl.n & 63 : 64;
+      for (int kb = 0; kb < tl.blocks; ++kb) {
+        // (lanes may disagree only once a wait has run out)
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->full[stage]), phase, wctx))) return;
+        if (kb + 1 == tl.blocks && valid < 64) {
+          const int vecs = (16 - (valid & 15)) * 8;  // 16-byte vectors of a 64-column chunk
+          const int chunks = 2 + (tl.nmma + 63) / 64;
+          for (int c = 0; c < chunks; ++c) {
+            const uint32_t base = (c < 2 ? sA + stage * a_bytes + c * 64 * kSpan : sB + stage * b_bytes + (c - 2) * 64 * kSpan) +
+                                  valid * kSpan;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (lane + 32 * v < vecs)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + (lane + 32 * v) * 16), "r"(0) : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bars->sf_full[stage]));
+        }
+        // (a stage is refilled only when this warp has passed it too: its waits never fall a turn behind)
+        if (lane == 0) mbar_arrive(smem_u32(&bars->empty[stage]));
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  };
+
   if (warp == 0) {
     if (elect_one()) produce(1);
     __syncwarp();
   } else if (warp == 1) {
-    if (leader) {
-      if (MODE == kDw) {
-        const bool one = elect_one();
-        multiply(one);
-      } else if (elect_one()) {
-        multiply(true);
-      }
-    }
+    if (leader && elect_one()) multiply();
     __syncwarp();
-  } else if (warp == 6) {
+  } else if (warp == 2 + kGroupEpi) {
     if (elect_one()) produce(2);
     __syncwarp();
-  } else if (MODE == kMx && warp == 7) {
+  } else if (MODE == kDw && warp == 3 + kGroupEpi) {
+    clear_edges();
+    __syncwarp();
+  } else if (MODE == kMx && warp == 3 + kGroupEpi) {
     if (elect_one()) copy_scales();
     __syncwarp();
+  } else if (MODE == kMx && warp == 4 + kGroupEpi) {
+    if (elect_one()) produce(4);
+    __syncwarp();
   } else {
+    // eight warps, two to each quarter of the TMEM lanes, which take its chunks of 32 columns in turn (with
+    // four the weight gradient waited for its accumulators)
     const int q = warp & 3;
+    const int half = warp >= 6;
+    const uint32_t stage_base = sEpi + (warp - 2) * kGroupStage;
+    // gives an accumulator back to the MMA warp
+    auto hand_back = [&](int acc) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2)
+          mbar_arrive_cluster(mapa(smem_u32(&bars->tmem_empty[acc]), 0));
+        else
+          mbar_arrive(smem_u32(&bars->tmem_empty[acc]));
+      }
+    };
+    // starts the load of this warp's next 32 columns, or hands the accumulator back behind its last ones
+    auto next_columns = [&](uint32_t t_addr, int c, int left, uint32_t (&v)[32], int acc) {
+      if (left > 64)
+        tmem_ld_32x32(t_addr + c + 64, v);
+      else
+        hand_back(acc);
+    };
     int acc = 0;
     uint32_t acc_phase = 0;
     int at = 0;
     GroupTile tl;
-    for (int t = first_tile; group_tile<MODE, CG>(p, groups, at, t, total, tl); t += tile_step) {
+    for (int i = 0; group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
       const bool empty = MODE == kDw && tl.blocks == 0;
       const int m = tl.m0 + static_cast<int>(cta_rank) * kTileM + q * 32 + lane;
       const bool mine = m < p.M;
@@ -495,43 +608,99 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         tc_fence_after();
       }
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * p.BN);
-      for (int c = 0; c < tl.ncols; c += 32) {
-        uint32_t v[32];
-        if (empty) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0u;
-        } else {
-          tmem_ld_32x32(t_addr + c, v);
-          tmem_ld_wait();
-          if (c + 32 >= tl.ncols) {  // last read of this accumulator
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (CG == 2)
-                mbar_arrive_cluster(mapa(smem_u32(&bars->tmem_empty[acc]), 0));
-              else
-                mbar_arrive(smem_u32(&bars->tmem_empty[acc]));
-            }
+      if (half && tl.ncols <= 32) {  // nothing for this warp
+        if (!empty) {
+          hand_back(acc);
+          if (++acc == p.acc_stages) {
+            acc = 0;
+            acc_phase ^= 1u;
           }
         }
+        continue;
+      }
+      if (!empty && tl.ncols <= 8) {
+        // few rows: the wide path's code would be fetched for eight columns (1.1 us a call of one token)
+        uint32_t v[8];
+        tmem_ld_32x8(t_addr, v);
+        tmem_ld_wait();
+        hand_back(acc);
         if (mine) {
-          const int left = tl.ncols - c;
-          const long long o = first + c * p.ldc;
-          if (p.out_type == 0) {
-            float* out = static_cast<float*>(p.out) + o;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < tl.ncols) {
+              if (p.out_type == 0)
+                static_cast<uint32_t*>(p.out)[first + j * p.ldc] = v[j];
+              else
+                static_cast<uint16_t*>(p.out)[first + j * p.ldc] = static_cast<uint16_t>(pack16(p.out_type, v[j], 0u));
+            }
+        }
+        if (++acc == p.acc_stages) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+        continue;
+      }
+      uint32_t v[32];
+      if (empty) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0u;
+      } else {
+        tmem_ld_32x32(t_addr + half * 32, v);
+      }
+      for (int c = half * 32; c < tl.ncols; c += 64) {
+        const int left = tl.ncols - c;
+        // (opaque here: multiples of the row pitch, computed once for all tiles, would take 64 registers
+        // and spill)
+        long long ldc = p.ldc;
+        asm volatile("" : "+l"(ldc));
+        const long long o = first + c * ldc;
+        if (p.out_type == 0) {
+          uint32_t w[32];
+          if (!empty) tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) w[j] = v[j];
+          if (!empty) next_columns(t_addr, c, left, v, acc);
+          if (mine) {
+            uint32_t* out = static_cast<uint32_t*>(p.out) + o;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < left) out[j * p.ldc] = __uint_as_float(v[j]);
-          } else if (p.out_type == 1) {
-            __half* out = static_cast<__half*>(p.out) + o;
+              if (j < left) out[j * ldc] = w[j];
+          }
+        } else {
+          uint32_t h[16];  // columns 2 j (low half) and 2 j + 1
+          if (!empty) tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) h[j] = pack16(p.out_type, v[2 * j], v[2 * j + 1]);
+          if (!empty) next_columns(t_addr, c, left, v, acc);
+          if (p.wide_rows) {
+            // through shared memory to 16-byte stores: the lane writes its 32 columns as 32 rows of 64
+            // bytes (16-byte pieces xor-swizzled by row pair), then four lanes store a row
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint32_t a = stage_base + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1))))
+                           : "memory");
+            }
+            __syncwarp();
+            const int piece = lane & 3;
+            const int mp = m - lane + piece * 8;  // (the extent is a multiple of 8: all of a piece or none)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = i * 8 + (lane >> 2);
+              uint4 d;
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(d.x), "=r"(d.y), "=r"(d.z), "=r"(d.w)
+                           : "r"(stage_base + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                           : "memory");
+              if (row < left && mp < p.M)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o - lane + piece * 8 + row * ldc) = d;
+            }
+            __syncwarp();
+          } else if (mine) {
+            uint16_t* out = static_cast<uint16_t*>(p.out) + o;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < left) out[j * p.ldc] = __float2half_rn(__uint_as_float(v[j]));
-          } else {
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + o;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < left) out[j * p.ldc] = __float2bfloat16_rn(__uint_as_float(v[j]));
+              if (j < left) out[j * ldc] = static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1)));
           }
         }
       }

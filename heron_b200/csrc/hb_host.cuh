@@ -388,7 +388,8 @@ struct hb_plan {
   // wide strip conv (conv_algo 3): channels on the MMA's M axis, up to 256 pixels on N
   bool strip_t;
   hb::StripTParams spt;
-  // products grouped by expert and 4-bit products: tmA, tmB (64-row boxes), tmB2 (16-row boxes);
+  // products grouped by expert and 4-bit products: tmA, and the token matrix in boxes of 64 rows (tmB), of 16
+  // (tmB2) and of a whole tile (tmC);
   // group_zero_bytes: no rows at all, the weight gradient is cleared and nothing is launched
   bool group;
   int group_mode;

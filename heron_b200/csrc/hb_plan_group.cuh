@@ -15,7 +15,7 @@ struct GroupProblem {
 };
 
 int group_fixed_smem(int E) {
-  return 1024 /*alignment of the ring*/ + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
+  return 1024 /*alignment of the ring*/ + hb::kGroupEpi * hb::kGroupStage + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
          E * static_cast<int>(sizeof(hb::GroupEntry));
 }
 
@@ -111,6 +111,7 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   p.out = out;
   p.out_type = out_type_of(g.out);
   p.ldc = g.M;
+  p.wide_rows = eo == 2 && g.M % 8 == 0;
   p.out_group = static_cast<long long>(g.C) * g.M;
   p.sfa = static_cast<const uint8_t*>(sfa);
   p.sfb = static_cast<const uint8_t*>(sfb);
@@ -134,6 +135,9 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   int units = d.sm_count / k.cta_group;
   if (k.max_ctas > 0 && k.max_ctas / k.cta_group < units) units = k.max_ctas / k.cta_group;
   if (units < 1) units = 1;
+  // (with fewer rows a group than the narrowest tiles hold all tiles cost the same; the sort takes about 1 us,
+  // which few tiles do not earn back: 777 rows in 20 groups 6.8 us without, 8.1 us with it)
+  p.sorted = tiles > 3LL * units && g.E > 1 && g.E <= hb::kSortedGroups && g.T / g.E >= 32;
   plan->grid = static_cast<int>(tiles < units ? tiles : units) * k.cta_group;
   plan->smem = group_fixed_smem(g.E) + k.stages * group_stage(g, k.tile_n, k.cta_group);
   plan->knobs = k;
@@ -144,15 +148,17 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
     rc = encode_tiled3(d, &plan->tmA, HB_U8, A, row, M, E, row, row * M, 128, hb::kTileM, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, HB_U8, B, row, T, 1, row, row * T, 128, 64, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB2, HB_U8, B, row, T, 1, row, row * T, 128, 16, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmC, HB_U8, B, row, T, 1, row, row * T, 128, k.tile_n, 128);
   } else if (dw) {
     rc = encode_tiled3(d, &plan->tmA, g.in, A, M, T, 1, M * 2, M * 2 * T, 64, 64, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, g.in, B, C, T, 1, C * 2, C * 2 * T, 64, 64, 128);
-    plan->tmB2 = plan->tmB;
+    plan->tmC = plan->tmB2 = plan->tmB;
   } else {
     rc = g.mode == hb::kFwd ? encode_tiled3(d, &plan->tmA, g.in, A, R, M, E, R * 2, R * 2 * M, 64, hb::kTileM, 128)
                             : encode_tiled3(d, &plan->tmA, g.in, A, M, R, E, M * 2, M * 2 * R, 64, 64, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, g.in, B, R, T, 1, R * 2, R * 2 * T, 64, 64, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB2, g.in, B, R, T, 1, R * 2, R * 2 * T, 64, 16, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmC, g.in, B, R, T, 1, R * 2, R * 2 * T, 64, k.tile_n / k.cta_group, 128);
   }
   return rc;
 }
@@ -198,7 +204,7 @@ int launch_group(const hb_plan* plan, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG>, plan->tmA, plan->tmB, plan->tmB2, plan->gp);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->gp);
   return e == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 

@@ -543,7 +543,33 @@ def plan_conv3d_ncdhw(x, w, stride=1, padding=0, out=None, out_dtype=None, scrat
 _WIDE_CODES = {torch.float16: _lib.HB_F16, torch.bfloat16: _lib.HB_BF16, torch.float32: _lib.HB_F32}
 
 # The small calls of these operators are bound by the host (a token's product takes the GPU a few
-# microseconds): one pass over the checks, addresses and streams as plain ints.
+# microseconds).  A call without knobs first goes to the C++ front end (csrc/hb_front.cpp), which checks,
+# allocates and launches in one step; what it finds unusual it hands back (None), and the code below
+# checks again, names the fault or does the call.
+class _Front:
+    """The extension module, loaded by the first call (importing this file loads nothing)."""
+
+    def __getattr__(self, name):
+        _lib.load()
+        try:
+            from . import _front
+        except ImportError as e:
+            raise ImportError("heron_b200/_front.so is not built or does not load (run `python -m "
+                              "heron_b200.build`): %s" % e)
+        for fn in ("grouped", "quantize", "dequantize", "mx"):
+            setattr(self, fn, getattr(_front, fn))
+        return getattr(_front, name)
+
+
+_fast = _Front()
+
+
+def _done(result, kind):
+    if result.__class__ is int:
+        _lib.check(result, kind)
+    return result
+
+
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -651,12 +677,20 @@ def grouped_gemm(x, w, offsets, out=None, out_dtype=None, knobs=None):
     read by the kernel, so a captured call may be replayed with other offsets).  float16 or bfloat16
     operands, fp32 accumulation, out float32 (default), float16 or bfloat16.  K % 8 == 0.  Rows of no
     group are left as they are in `out` (arbitrary in a fresh one)."""
+    if knobs is None:
+        done = _fast.grouped(0, x, w, offsets, out, out_dtype)
+        if done is not None:
+            return _done(done, "hb_grouped_gemm")
     tensors, sizes = _grouped_args("hb_grouped_gemm", x, w, offsets, out, out_dtype)
     return _run("hb_grouped_gemm", tensors, sizes, knobs, tensors[2])
 
 
 def grouped_gemm_dx(dy, w, offsets, out=None, out_dtype=None, knobs=None):
     """Gradient of grouped_gemm's rows: out[r] = w[e]^T @ dy[r]; dy (T,N), out (T,K).  N % 8 == K % 8 == 0."""
+    if knobs is None:
+        done = _fast.grouped(1, dy, w, offsets, out, out_dtype)
+        if done is not None:
+            return _done(done, "hb_grouped_gemm_dx")
     tensors, sizes = _grouped_args("hb_grouped_gemm_dx", dy, w, offsets, out, out_dtype)
     return _run("hb_grouped_gemm_dx", tensors, sizes, knobs, tensors[2])
 
@@ -664,6 +698,10 @@ def grouped_gemm_dx(dy, w, offsets, out=None, out_dtype=None, knobs=None):
 def grouped_gemm_dw(dy, x, offsets, out=None, out_dtype=None, knobs=None):
     """Gradient of grouped_gemm's weights: out[e] = sum of dy[r] x[r]^T over the rows of group e, zeros
     for a group without rows; dy (T,N), x (T,K), out (E,N,K).  N % 8 == K % 8 == 0."""
+    if knobs is None:
+        done = _fast.grouped(2, dy, x, offsets, out, out_dtype)
+        if done is not None:
+            return _done(done, "hb_grouped_gemm_dw")
     tensors, sizes = _grouped_args("hb_grouped_gemm_dw", dy, x, offsets, out, out_dtype)
     return _run("hb_grouped_gemm_dw", tensors, sizes, knobs, tensors[2])
 
@@ -725,6 +763,9 @@ def quantize_mxfp4(x, offsets=None, codes=None, scales=None):
     codes has x's shape with K / 2; scales is (mxfp4_scale_bytes(...),), for a batch (batch, ...).  With
     `offsets` the rows belong to groups, as grouped_gemm_mxfp4 takes them; rows of no group are skipped.
     K % 32 == 0."""
+    done = _fast.quantize(x, offsets, codes, scales)
+    if done is not None:
+        return _done(done, "hb_quantize_mxfp4")
     shape = x.shape
     K = shape[-1] if shape else 0
     code = _wide_code(x.dtype)
@@ -744,6 +785,9 @@ def quantize_mxfp4(x, offsets=None, codes=None, scales=None):
 
 def dequantize_mxfp4(codes, scales, offsets=None, out=None, out_dtype=None):
     """The values that quantize_mxfp4's result stands for, float32 (default), bfloat16 or float16."""
+    done = _fast.dequantize(codes, scales, offsets, out, out_dtype)
+    if done is not None:
+        return _done(done, "hb_dequantize_mxfp4")
     shape = codes.shape
     K = 2 * shape[-1] if shape else 0
     batch, rows, groups, scale_shape = _mx_shape(codes, K, offsets, "codes")
@@ -786,6 +830,10 @@ def gemm_mxfp4(a, a_scales, b, b_scales, out=None, out_dtype=None, knobs=None):
     """out[M,N] = sum_k a[m,k] * b[n,k] over the values that two quantised matrices stand for:
     a (M, K/2) and b (N, K/2) with the scales quantize_mxfp4 gave; out float32 (default), float16 or
     bfloat16, fp32 accumulation."""
+    if knobs is None:
+        done = _fast.mx(a, a_scales, b, b_scales, None, out, out_dtype)
+        if done is not None:
+            return _done(done, "hb_gemm_mxfp4")
     tensors, sizes = _mx_args(a, a_scales, b, b_scales, None, out, out_dtype)
     return _run("hb_gemm_mxfp4", tensors, sizes, knobs, tensors[4])
 
@@ -794,6 +842,10 @@ def grouped_gemm_mxfp4(x, x_scales, w, w_scales, offsets, out=None, out_dtype=No
     """grouped_gemm over quantised operands: x (T, K/2) quantised with the same offsets, w (E, N, K/2)
     quantised as a batch."""
     _needs_offsets(offsets)
+    if knobs is None:
+        done = _fast.mx(x, x_scales, w, w_scales, offsets, out, out_dtype)
+        if done is not None:
+            return _done(done, "hb_grouped_gemm_mxfp4")
     tensors, sizes = _mx_args(x, x_scales, w, w_scales, offsets, out, out_dtype)
     return _run("hb_grouped_gemm_mxfp4", tensors, sizes, knobs, tensors[4])
 
