@@ -61,6 +61,7 @@ struct GroupParams {
   int stages, acc_stages, tmem_cols, tiles_m;
   int out_type;         // 0: fp32, 1: fp16, 2: bf16
   int wide_rows;        // 16-bit output whose rows are multiples of 16 bytes
+  int ksplit;           // SPLIT: CTAs of a cluster that share a tile's reduction
   int sorted;           // more tiles than CTAs: groups in order of their tiles' cost, see group_list
   uint32_t idesc;       // without the N field
   void* out;
@@ -83,6 +84,7 @@ struct GroupTile {
   int c0, ncols;    // first column within the group (kDw: of the column axis) and valid columns
   int nmma;         // columns the MMA computes
   int blocks;       // reduction blocks
+  int kb0, kb1;     // those of this CTA
 };
 
 __host__ __device__ __forceinline__ int round_up(int v, int step) { return (v + step - 1) / step * step; }
@@ -198,6 +200,7 @@ struct GroupBars {
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
   uint64_t drain, sf_drain;
+  uint64_t red_full, red_empty;  // SPLIT: a share's partial sums are here; are read
   uint32_t tmem_base;
   int abort_flag;
   int total;
@@ -221,7 +224,7 @@ __device__ __forceinline__ uint32_t pack16(int out_type, uint32_t a, uint32_t b)
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int MODE, int CG>
+template <int MODE, int CG, bool SPLIT = false>
 __global__ void __launch_bounds__(group_threads(MODE), 1)
 hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ CUtensorMap tmBw,
@@ -232,6 +235,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  static_assert(!SPLIT || (CG == 1 && (MODE == kFwd || MODE == kMx)), "the joined form is that of the forward products");
   const uint32_t cta_rank = (CG == 2) ? cluster_ctarank() : 0u;
   const bool leader = cta_rank == 0u;
   constexpr int a_bytes = kTileM * kSpan;
@@ -245,6 +249,10 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   uint8_t* after = smem + (sEpi - smem_base) + kGroupEpi * kGroupStage;
   GroupBars* bars = reinterpret_cast<GroupBars*>(after);
   GroupEntry* groups = reinterpret_cast<GroupEntry*>(after + ((sizeof(GroupBars) + 15) & ~15));
+  // SPLIT: partial sums of this CTA's share of the lanes, [source][column][lane]
+  const int ks = SPLIT ? p.ksplit : 1;
+  const int ks_rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  float* const red = reinterpret_cast<float*>(groups + p.E);
   volatile int* abort_flag = &bars->abort_flag;
   const WaitCtx wctx{abort_flag, p.wait_limit_cycles > 0 ? p.wait_limit_cycles : HB_WAIT_LIMIT_CYCLES};
   const int warp = threadIdx.x >> 5;
@@ -262,6 +270,10 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
     mbar_init(smem_u32(&bars->drain), 1);
     mbar_init(smem_u32(&bars->sf_drain), 1);
+    if (SPLIT) {
+      mbar_init(smem_u32(&bars->red_full), ks * 2 * max(4 / ks, 1));  // two warps of each quarter of the lanes in a share
+      mbar_init(smem_u32(&bars->red_empty), ks * kGroupEpi);
+    }
     bars->abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmA);
@@ -270,18 +282,25 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (warp == 1) tmem_alloc_cg<CG>(smem_u32(&bars->tmem_base), static_cast<uint32_t>(p.tmem_cols));
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync();
+  if (CG == 2 || SPLIT) cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
   griddep_wait();  // (the offsets too may come from the kernel before)
   griddep_launch_dependents();
   const int total = group_list<MODE, CG>(p, groups, &bars->total);
-  const int first_tile = blockIdx.x / CG;
-  const int tile_step = gridDim.x / CG;
+  const int first_tile = blockIdx.x / (CG * ks);
+  const int tile_step = gridDim.x / (CG * ks);
 
   // the i-th tile of this CTA (pair)
   auto tile_of = [&](int i) {
     return i * tile_step + (p.sorted && (i & 1) ? tile_step - 1 - first_tile : first_tile);
+  };
+
+  auto take = [&](int& at, int i, GroupTile& tl) {
+    if (!group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl)) return false;
+    tl.kb0 = SPLIT ? ks_rank * tl.blocks / ks : 0;
+    tl.kb1 = SPLIT ? (ks_rank + 1) * tl.blocks / ks : tl.blocks;
+    return true;
   };
 
   // B rows (K-major) or columns (MN-major) of a tile that this CTA stages, and how they are fetched: boxes
@@ -305,7 +324,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     int at = 0;
     GroupTile tl;
     const int kt = MODE == kMx ? (p.R + 127) / 128 : 0;  // scale tiles along the reduction
-    for (int i = 0; ok && !p.silent_producer && group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
+    for (int i = 0; ok && !p.silent_producer && take(at, i, tl); ++i) {
       int box;
       const int boxes = b_boxes(tl.nmma, box);
       const uint32_t tx_ab = static_cast<uint32_t>(a_bytes + boxes * box * kSpan) * CG;
@@ -318,7 +337,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         sfa = p.sfa + (static_cast<long long>(tl.e) * p.tiles_m + tl.m0 / kTileM) * kt * kAtomBytes;
         sfb = p.sfb + (static_cast<long long>(tl.start / 128 + tl.e + tl.c0 / 128)) * kt * kAtomBytes;
       }
-      for (int kb = 0; kb < tl.blocks; ++kb) {
+      for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
         const uint32_t full_local = smem_u32(&bars->full[stage]);
         const uint32_t full = (CG == 2) ? mapa(full_local, 0) : full_local;
         if (!mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, wctx)) {
@@ -405,15 +424,15 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
     int at = 0;
     GroupTile tl;
-    for (int i = 0; ok && group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
-      if (MODE == kDw && tl.blocks == 0) continue;  // (the epilogue writes zeros without an accumulator)
+    for (int i = 0; ok && take(at, i, tl); ++i) {
+      if ((MODE == kDw || SPLIT) && tl.kb0 == tl.kb1) continue;  // (the epilogue writes zeros without an accumulator)
       ok = mbar_wait(smem_u32(&bars->tmem_empty[acc]), acc_phase ^ 1u, wctx);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * p.BN);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tl.nmma >> 3) << 17);
       uint32_t accum = 0u;
-      for (int kb = 0; kb < tl.blocks; ++kb) {
+      for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
         ok = mbar_wait(full0 + 8u * stage, phase, wctx);
         if (MODE == kMx && ok) ok = mbar_wait(sf_full0 + 8u * stage, phase, wctx);
         if (!ok) break;
@@ -486,9 +505,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
     int at = 0;
     GroupTile tl;
-    for (int i = 0; ok && group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
+    for (int i = 0; ok && take(at, i, tl); ++i) {
       const int nb_sf = sf_b_rows(tl);
-      for (int kb = 0; kb < tl.blocks; ++kb) {
+      for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
         if (!mbar_wait(smem_u32(&bars->full[stage]), phase, wctx)) {
           ok = false;
           break;
@@ -521,9 +540,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     int stage = 0, at = 0;
     uint32_t phase = 0;
     GroupTile tl;
-    for (int i = 0; group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
+    for (int i = 0; take(at, i, tl); ++i) {
       const int valid = tl.n & 15 ? tl.n & 63 : 64;
-      for (int kb = 0; kb < tl.blocks; ++kb) {
+      for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
         // (lanes may disagree only once a wait has run out)
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->full[stage]), phase, wctx))) return;
         if (kb + 1 == tl.blocks && valid < 64) {
@@ -597,8 +616,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     uint32_t acc_phase = 0;
     int at = 0;
     GroupTile tl;
-    for (int i = 0; group_tile<MODE, CG>(p, groups, at, tile_of(i), total, tl); ++i) {
-      const bool empty = MODE == kDw && tl.blocks == 0;
+    uint32_t red_phase = 0;
+    for (int i = 0; take(at, i, tl); ++i) {
+      const bool empty = (MODE == kDw || SPLIT) && tl.kb0 == tl.kb1;
       const int m = tl.m0 + static_cast<int>(cta_rank) * kTileM + q * 32 + lane;
       const bool mine = m < p.M;
       const long long row0 = MODE == kDw ? tl.c0 : static_cast<long long>(tl.start) + tl.c0;
@@ -608,6 +628,56 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         tc_fence_after();
       }
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * p.BN);
+      if constexpr (SPLIT) {
+        // Every CTA of the cluster has the sums over its share of the reduction.  CTA j joins lanes
+        // [j L, (j + 1) L), L = 128 / ks: the others write theirs into its buffer, it adds them in the order
+        // of the shares and stores the result.
+        const int share = kTileM / ks;
+        uint32_t v[32];
+        if (empty) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0u;
+        } else {
+          tmem_ld_32x32(t_addr + half * 32, v);
+          tmem_ld_wait();
+          hand_back(acc);
+          if (++acc == p.acc_stages) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+        }
+        // (the buffers are free again once every share of the tile before has been read)
+        if (!mbar_wait_cluster(smem_u32(&bars->red_empty), red_phase ^ 1u, wctx)) break;
+        const int at_lane = q * 32 + lane, owner = at_lane / share;
+        const uint32_t dst = mapa(smem_u32(red), owner) +
+                             ((ks_rank * 64 + half * 32) * share + at_lane - owner * share) * 4;
+        const int mine_cols = min(tl.ncols - half * 32, 32);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < mine_cols) st_cluster_u32(dst + j * share * 4, v[j]);
+        __syncwarp();
+        const int first_owner = q * 32 / share, last_owner = (q * 32 + 31) / share;
+        if (lane <= last_owner - first_owner)
+          mbar_arrive_cluster(mapa(smem_u32(&bars->red_full), first_owner + lane));
+        if (!mbar_wait_cluster(smem_u32(&bars->red_full), red_phase, wctx)) break;
+        const int m0 = tl.m0 + ks_rank * share;
+        for (int u = threadIdx.x - 64; u < share * tl.ncols; u += kGroupEpi * 32) {
+          const int col = u / share, l = u - col * share;
+          float sum = 0.f;
+          for (int k = 0; k < ks; ++k) sum += red[(k * 64 + col) * share + l];
+          if (m0 + l < p.M) {
+            const long long o = (static_cast<long long>(tl.start) + tl.c0 + col) * p.ldc + m0 + l;
+            if (p.out_type == 0)
+              static_cast<float*>(p.out)[o] = sum;
+            else
+              static_cast<uint16_t*>(p.out)[o] = static_cast<uint16_t>(pack16(p.out_type, __float_as_uint(sum), 0u));
+          }
+        }
+        __syncwarp();
+        if (lane < ks) mbar_arrive_cluster(mapa(smem_u32(&bars->red_empty), lane));
+        red_phase ^= 1u;
+        continue;
+      }
       if (half && tl.ncols <= 32) {  // nothing for this warp
         if (!empty) {
           hand_back(acc);
@@ -714,7 +784,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync();
+  if (CG == 2 || SPLIT) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_cg<CG>(tmem_base, static_cast<uint32_t>(p.tmem_cols));

@@ -11,6 +11,7 @@
 #include "hb_conv_strip_t.cuh"
 #include "hb_group.cuh"
 #include "hb_mx.cuh"
+#include "hb_rows.cuh"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -57,7 +58,9 @@ bool setup_device(Driver* d) {
   if (prop.major != 10) return false;
   d->sm_count = prop.multiProcessorCount;
   // Opt in to the large dynamic shared-memory carve-out for every kernel instantiation.
-  const void* kernels[37] = {
+  const void* kernels[39] = {
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1, true>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 1, true>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 2>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kDx, 1>),
@@ -395,6 +398,8 @@ struct hb_plan {
   int group_mode;
   hb::GroupParams gp;
   size_t group_zero_bytes;
+  bool group_rows;  // few rows: the kernels of hb_rows.cuh on rp instead
+  hb::RowsParams rp;
   // NCHW operators only: one launch that brings input and filter to NHWC / HWIO first (the conv
   // kernel's epilogue writes NCHW itself)
   bool has_pre, pre_is_stem;

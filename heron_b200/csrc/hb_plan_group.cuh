@@ -14,9 +14,18 @@ struct GroupProblem {
   hb_dtype in, out;  // in: unused for kMx
 };
 
-int group_fixed_smem(int E) {
-  return 1024 /*alignment of the ring*/ + hb::kGroupEpi * hb::kGroupStage + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
+// (split: the buffer in which the CTAs of a cluster join their sums, 128 lanes x 64 columns)
+int group_fixed_smem(int E, bool split = false) {
+  return (split ? hb::kTileM * 64 * 4 : 0) + 1024 /*alignment of the ring*/ + hb::kGroupEpi * hb::kGroupStage + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
          E * static_cast<int>(sizeof(hb::GroupEntry));
+}
+
+// Most tiles that the offsets can ask for.
+long long most_tiles(const GroupProblem& g, const hb_knobs& k) {
+  const int rows_m = hb::kTileM * k.cta_group;
+  const long long ct = g.mode == hb::kDw ? static_cast<long long>(g.E) * ((g.C + k.tile_n - 1) / k.tile_n)
+                                         : (g.T < g.T / k.tile_n + g.E ? g.T : g.T / k.tile_n + g.E);
+  return ct * ((g.M + rows_m - 1) / rows_m);
 }
 
 int group_stage(const GroupProblem& g, int BN, int cg) {
@@ -44,7 +53,21 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
     else
       k.tile_n = k.cta_group == 2 || avg > 96 ? 256 : (avg > 48 ? 128 : 64);
   }
-  const int room = kSmemLimit - group_fixed_smem(g.E);
+  if (k.split_k == 0) {
+    // A product of few tiles: the reduction of a tile over a cluster of 2 or 4 CTAs, as long as all of them
+    // find an SM.  A tile's time is that of its operands through one SM's ring; the cluster costs about 2 us.
+    // Measured, one against four CTAs a tile: 64 rows x 4096 features, bf16, K 4096 17.6 / 14.5 us, 32 rows
+    // 18.5 / 12.1; MXFP4 32 rows, K 8192 15.1 / 11.4, K 4096 (16 blocks) 9.6 / 10.0.  (Clusters of eight: 128
+    // CTAs did not all run at once, 12.3 us where four took 7.8.)
+    k.split_k = 1;
+    if ((g.mode == hb::kFwd || g.mode == hb::kMx) && k.cta_group == 1 && k.tile_n == 64) {
+      const int elems = g.mode == hb::kMx ? 256 : 64;
+      const int sms = k.max_ctas > 0 && k.max_ctas < 148 ? k.max_ctas : 148;
+      if ((g.R + elems - 1) / elems >= 32)
+        while (k.split_k < 4 && most_tiles(g, k) * k.split_k * 2 <= sms) k.split_k *= 2;
+    }
+  }
+  const int room = kSmemLimit - group_fixed_smem(g.E, k.split_k > 1);
   if (k.stages == 0) {
     k.stages = room / group_stage(g, k.tile_n, k.cta_group);
     const int most = g.mode == hb::kMx ? (512 - k.tile_n) / (8 * (1 + hb::group_sf_rows(k.tile_n))) : hb::kMaxStages;
@@ -69,8 +92,28 @@ int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
   if (k.acc_stages < 1 || k.acc_stages > 2) return HB_ERR_KNOB;
   if (k.max_ctas < 0) return HB_ERR_KNOB;
   if (group_tmem(g, k) > 512) return HB_ERR_KNOB;
-  if (group_fixed_smem(g.E) + k.stages * group_stage(g, k.tile_n, k.cta_group) > kSmemLimit) return HB_ERR_KNOB;
+  if (k.split_k != 1 && k.split_k != 2 && k.split_k != 4 && k.split_k != 8) return HB_ERR_KNOB;
+  if (k.split_k > 1 && (k.cta_group != 1 || k.tile_n != 64 || (g.mode != hb::kFwd && g.mode != hb::kMx))) return HB_ERR_KNOB;
+  if (group_fixed_smem(g.E, k.split_k > 1) + k.stages * group_stage(g, k.tile_n, k.cta_group) > kSmemLimit) return HB_ERR_KNOB;
   return HB_OK;
+}
+
+// Whether a product is left to the kernels that stream the weights (hb_rows.cuh).  Measured against the tile
+// kernel: bf16, 1 and 8 rows x 4096 x 4096 7.0 and 8.4 / 17.0 us (with its reduction over a cluster 10.4), 16
+// rows (two passes) 16.9 / 11; 16 and 32 rows over 32 experts of 2048 x 2048 20.8 and 30.8 / 22.6 and 32.9, 16 rows
+// over 8 13.9 / 13.1.  MXFP4, whose kernel is bound by widening elements, by the weights of all passes: 16.8
+// million 6.9 / 9.3 us (one row, 4096 x 4096) and 7.0 / 7.1 (four rows to four experts of 2048 x 2048), twice as
+// many 10.2 / 7.4; and a long reduction over few features is one for the cluster (1024 x 16384 13 / 8.4).
+bool few_rows(const GroupProblem& g) {
+  if (g.mode == hb::kFwd) return g.T <= (g.E > 8 ? g.E : 8);
+  if (g.mode != hb::kMx || g.T > 64 || g.R > 8192) return false;
+  const long long passes = g.E == 1 ? (g.T + 7) / 8 : g.T;
+  return passes * g.M * g.R <= (1LL << 24);
+}
+
+// Knobs of the tile kernel, given by the caller: then that kernel is meant.
+bool knob_names_tiles(const hb_knobs& k) {
+  return k.tile_n || k.split_k || k.stages || k.acc_stages || k.max_ctas || k.cta_group || k.silent_producer;
 }
 
 // A: w (kFwd, kDx, kMx) or x (kDw); B: the token matrix (kDw: dy).
@@ -100,6 +143,21 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   group_knobs(g, knobs, &k);
   int rc = check_group_knobs(g, k);
   if (rc != HB_OK) return rc;
+  if ((!knobs || !knob_names_tiles(*knobs)) && few_rows(g)) {
+    hb::RowsParams& r = plan->rp;
+    r.w = A; r.x = B; r.out = out; r.offsets = offsets;
+    r.w_sf = static_cast<const uint8_t*>(sfa);
+    r.x_sf = static_cast<const uint8_t*>(sfb);
+    r.E = g.E; r.T = g.T; r.N = g.M; r.K = g.R;
+    r.out_type = out_type_of(g.out);
+    r.w_matrix_sf = mx ? (g.M + 127LL) / 128 * ((g.R + 127LL) / 128) * hb::kAtomBytes : 0;
+    plan->group_rows = true;
+    plan->group_mode = mx ? hb::kMx : (g.in == HB_F16 ? 1 : 2);
+    plan->knobs = k;
+    // (4-bit: 16 features to a block within a tile of 128)
+    plan->grid = mx ? (g.M + 127) / 128 * 8 : (g.M + hb::kRowsFeatures - 1) / hb::kRowsFeatures;
+    return HB_OK;
+  }
 
   hb::GroupParams& p = plan->gp;
   p.offsets = offsets;
@@ -127,19 +185,18 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
     if (g.mode != hb::kFwd) p.idesc |= 1u << 15;
     if (dw) p.idesc |= 1u << 16;
   }
-  // most tiles the offsets can ask for
-  const long long ct = dw ? static_cast<long long>(g.E) * ((g.C + k.tile_n - 1) / k.tile_n)
-                          : (g.T < g.T / k.tile_n + g.E ? g.T : g.T / k.tile_n + g.E);
-  const long long tiles = ct * p.tiles_m;
+  const long long tiles = most_tiles(g, k);
   if (tiles > 0x3fffffffLL) return HB_ERR_SHAPE;
-  int units = d.sm_count / k.cta_group;
-  if (k.max_ctas > 0 && k.max_ctas / k.cta_group < units) units = k.max_ctas / k.cta_group;
+  const int together = k.cta_group * k.split_k;  // CTAs of a cluster
+  int units = d.sm_count / together;
+  if (k.max_ctas > 0 && k.max_ctas / together < units) units = k.max_ctas / together;
   if (units < 1) units = 1;
   // (with fewer rows a group than the narrowest tiles hold all tiles cost the same; the sort takes about 1 us,
   // which few tiles do not earn back: 777 rows in 20 groups 6.8 us without, 8.1 us with it)
   p.sorted = tiles > 3LL * units && g.E > 1 && g.E <= hb::kSortedGroups && g.T / g.E >= 32;
-  plan->grid = static_cast<int>(tiles < units ? tiles : units) * k.cta_group;
-  plan->smem = group_fixed_smem(g.E) + k.stages * group_stage(g, k.tile_n, k.cta_group);
+  plan->grid = static_cast<int>(tiles < units ? tiles : units) * together;
+  p.ksplit = k.split_k;
+  plan->smem = group_fixed_smem(g.E, k.split_k > 1) + k.stages * group_stage(g, k.tile_n, k.cta_group);
   plan->knobs = k;
 
   const uint64_t T = g.T, E = g.E, M = g.M, R = g.R, C = g.C;
@@ -189,7 +246,7 @@ int plan_mx(const void* x, const void* x_scales, const void* w, const void* w_sc
   return plan_group(g, w, x, out, w_scales, x_scales, offsets, knobs, plan);
 }
 
-template <int MODE, int CG>
+template <int MODE, int CG, bool SPLIT = false>
 int launch_group(const hb_plan* plan, cudaStream_t stream) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
@@ -199,20 +256,44 @@ int launch_group(const hb_plan* plan, cudaStream_t stream) {
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = SPLIT ? plan->gp.ksplit : CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->gp);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG, SPLIT>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->gp);
   return e == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
+int launch_rows(const hb_plan* plan, cudaStream_t stream) {
+  const bool mx = plan->group_mode == hb::kMx;
+  const int warps = !mx && plan->rp.K > 2048 ? 16 : hb::kRowsWarps;
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(plan->grid, plan->rp.T);
+  cfg.blockDim = dim3(warps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  void (*kernel)(const hb::RowsParams) =
+      mx ? hb::hb_mx_rows_kernel
+         : (plan->group_mode == 1 ? (warps == 16 ? hb::hb_group_rows_kernel<1, 16> : hb::hb_group_rows_kernel<1, 8>)
+                                  : (warps == 16 ? hb::hb_group_rows_kernel<2, 16> : hb::hb_group_rows_kernel<2, 8>));
+  return cudaLaunchKernelEx(&cfg, kernel, plan->rp) == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+}
+
 int run_group(const hb_plan* plan, cudaStream_t stream) {
+  if (plan->group_rows) return launch_rows(plan, stream);
   if (plan->group_zero_bytes)
     return cudaMemsetAsync(plan->gp.out, 0, plan->group_zero_bytes, stream) == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
   if (plan->grid == 0) return HB_OK;  // no rows
   const bool pair = plan->knobs.cta_group == 2;
+  if (plan->gp.ksplit > 1)
+    return plan->group_mode == hb::kFwd ? launch_group<hb::kFwd, 1, true>(plan, stream)
+                                        : launch_group<hb::kMx, 1, true>(plan, stream);
   switch (plan->group_mode) {
     case hb::kFwd: return pair ? launch_group<hb::kFwd, 2>(plan, stream) : launch_group<hb::kFwd, 1>(plan, stream);
     case hb::kDx: return pair ? launch_group<hb::kDx, 2>(plan, stream) : launch_group<hb::kDx, 1>(plan, stream);

@@ -295,6 +295,37 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
                : "memory");
 }
 
+// A 32-bit store into the shared memory of a CTA of the cluster.
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+// The bounded wait on an mbarrier whose arrivals come from other CTAs of the cluster (acquire at cluster scope).
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, const WaitCtx& w) {
+  volatile int* abort_flag = w.abort_flag;
+  const long long t0 = clock64();
+  uint32_t polls = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((++polls & 63u) == 0u) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > w.limit_cycles) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
 // ---- cta_group-generic forms --------------------------------------------------------------
 // CG = 1: one CTA owns the MMA.  CG = 2: the two CTAs of a cluster share it; loads of either CTA
 // complete on the leader's mbarrier (`bar` is then a shared::cluster address).

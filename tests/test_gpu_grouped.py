@@ -103,6 +103,36 @@ def test_knobs_do_not_change_the_product(K, knobs):
         assert_product(K.grouped_gemm_dw(dy, x, offsets, knobs=knobs), want, mag, 514, "dw")
 
 
+@pytest.mark.parametrize("split", [2, 4, 8])
+@pytest.mark.parametrize("counts", ["decode", "uneven", "tile_edges", "empty"])
+@pytest.mark.parametrize("k,n", [(8, 40), (520, 264), (1024, 1001)])
+def test_a_reduction_over_a_cluster(K, split, counts, k, n):
+    c = COUNTS[counts]
+    x, w, _, off, offsets = make(split, c, 2, 3, k, n, torch.bfloat16)
+    want, mag, own = grouped(clean(x), w, off)
+    for od in (torch.float32, torch.bfloat16):
+        for extra in (dict(), dict(max_ctas=2 * split), dict(stages=1)):
+            out = torch.full((x.shape[0], n), 7.0, dtype=od, device="cuda")
+            K.grouped_gemm(x, w, offsets, out=out, knobs=dict(tile_n=64, split_k=split, **extra))
+            assert_product(out[own], want[own], mag[own], k, str(extra))
+            assert (out[~own] == 7.0).all()
+
+
+@pytest.mark.parametrize("T,E", [(1, 1), (1, 64), (5, 3), (8, 1), (9, 1), (16, 2), (40, 40), (64, 100)])
+@pytest.mark.parametrize("k,n", [(8, 1), (264, 40), (2056, 17), (4096, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_few_rows(K, T, E, k, n, dtype):
+    g = torch.Generator().manual_seed(T * E + k)
+    c = torch.bincount(torch.randint(0, E, (T,), generator=g), minlength=E).tolist()
+    x, w, _, off, offsets = make(T + k, c, 1, 1, k, n, dtype)
+    want, mag, own = grouped(clean(x), w, off)
+    for od in (torch.float32, dtype):
+        out = torch.full((T + 2, n), 7.0, dtype=od, device="cuda")
+        K.grouped_gemm(x, w, offsets, out=out)
+        assert_product(out[own], want[own], mag[own], k)
+        assert (out[~own] == 7.0).all()
+
+
 def test_an_infinity_stays_in_its_group(K):
     x, w, dy, off, offsets = make(3, [5, 9, 20], 0, 0, 64, 64, torch.float16)
     x[6], dy[6] = torch.inf, torch.nan

@@ -144,6 +144,14 @@ def test_product_knobs(K, knobs):
     product(K, 130, 200, 160, 12, torch.float32, knobs)
 
 
+@pytest.mark.parametrize("split", [2, 4, 8])
+@pytest.mark.parametrize("M,N,k", [(1, 1, 32), (3, 200, 1056), (64, 130, 2048), (130, 300, 800)])
+def test_a_reduction_over_a_cluster(K, split, M, N, k):
+    for od in (torch.float32, torch.bfloat16):
+        product(K, M, N, k, split, od, dict(tile_n=64, split_k=split))
+        product(K, M, N, k, split, od, dict(tile_n=64, split_k=split, max_ctas=split, stages=2))
+
+
 def test_product_of_single_elements(K):
     """One non-zero element a row: every (row, k) place of codes and scales meets its partner and no other."""
     k = 512
@@ -151,6 +159,24 @@ def test_product_of_single_elements(K):
     i = torch.arange(256, device="cuda")
     a[i, (i * 37 + 5) % k] = 2.0 ** (i % 9 - 4).float() * 1.5
     b[i, (i * 53 + 7) % k] = 2.0 ** (i % 7 - 3).float() * 3.0
+    out = K.gemm_mxfp4(*K.quantize_mxfp4(a), *K.quantize_mxfp4(b))
+    assert torch.equal(out.double(), a.double() @ b.double().T)
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 13, 40])
+@pytest.mark.parametrize("k", [32, 96, 1024])
+def test_sums_of_blocks_are_exact(K, M, k):
+    """With scales of 1 every sum of products is a multiple of 1/4 below 2^24 quarters: no bit may be lost."""
+    g = torch.Generator(device="cuda").manual_seed(M * k)
+    grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], device="cuda")
+
+    def operand(rows):
+        v = grid[torch.randint(0, 8, (rows, k), generator=g, device="cuda")]
+        v = v * (torch.randint(0, 4, (rows, k), generator=g, device="cuda") * 2 - 1).clamp(-1, 1)
+        v[0] = 6.0  # the largest sum there is
+        v[:, ::32] = 4.0  # (sets the block's scale to 1)
+        return v
+    a, b = operand(M), operand(150)
     out = K.gemm_mxfp4(*K.quantize_mxfp4(a), *K.quantize_mxfp4(b))
     assert torch.equal(out.double(), a.double() @ b.double().T)
 
