@@ -47,7 +47,7 @@ constexpr int kSortedGroups = 224;  // a thread each
 // scales and their producer
 constexpr int kGroupEpi = 8;
 __host__ __device__ constexpr int group_threads(int mode) { return 32 * (3 + kGroupEpi + (mode == kMx ? 2 : (mode == kDw ? 1 : 0))); }
-constexpr int kGroupStage = 2048;      // epilogue staging of a warp: 32 columns x 32 16-bit values
+constexpr int kGroupStage = 4096;      // epilogue staging of a warp: 2 x 32 columns x 32 16-bit values
 constexpr int kSpan = 128;             // bytes of the reduction axis in a ring stage (TMA swizzle span)
 constexpr int kAtomBytes = 512;        // scales of 128 rows x 128 elements
 
@@ -114,7 +114,7 @@ __device__ __forceinline__ bool group_tile(const GroupParams& p, const GroupEntr
   const int r = t - first;
   const int mt = r / ct;
   o.m0 = mt * kTileM * CG;
-  const int w = MODE == kDw ? p.BN : group_width<MODE, CG>(cols, ct, p.BN);
+  const int w = group_width<MODE, CG>(cols, ct, p.BN);
   o.c0 = (r - mt * ct) * w;
   o.ncols = min(w, cols - o.c0);
   o.nmma = round_up(o.ncols, 16 * CG);
@@ -605,13 +605,6 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           mbar_arrive(smem_u32(&bars->tmem_empty[acc]));
       }
     };
-    // starts the load of this warp's next 32 columns, or hands the accumulator back behind its last ones
-    auto next_columns = [&](uint32_t t_addr, int c, int left, uint32_t (&v)[32], int acc) {
-      if (left > 64)
-        tmem_ld_32x32(t_addr + c + 64, v);
-      else
-        hand_back(acc);
-    };
     int acc = 0;
     uint32_t acc_phase = 0;
     int at = 0;
@@ -710,67 +703,90 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
         continue;
       }
-      uint32_t v[32];
-      if (empty) {
+      // two of this warp's chunks of 32 columns at a time, 64 columns apart: the latencies of one (TMEM,
+      // shared memory) pass under the other's
+      for (int c = half * 32; c < tl.ncols; c += 128) {
+        const bool two = c + 64 < tl.ncols;
+        uint32_t v[2][32];
+        if (empty) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0u;
-      } else {
-        tmem_ld_32x32(t_addr + half * 32, v);
-      }
-      for (int c = half * 32; c < tl.ncols; c += 64) {
-        const int left = tl.ncols - c;
+          for (int j = 0; j < 32; ++j) v[0][j] = v[1][j] = 0u;
+        } else {
+          tmem_ld_32x32(t_addr + c, v[0]);
+          if (two) tmem_ld_32x32(t_addr + c + 64, v[1]);
+          tmem_ld_wait();
+          if (c + 128 >= tl.ncols) hand_back(acc);  // last read of this accumulator
+        }
         // (opaque here: multiples of the row pitch, computed once for all tiles, would take 64 registers
         // and spill)
         long long ldc = p.ldc;
         asm volatile("" : "+l"(ldc));
-        const long long o = first + c * ldc;
         if (p.out_type == 0) {
-          uint32_t w[32];
-          if (!empty) tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) w[j] = v[j];
-          if (!empty) next_columns(t_addr, c, left, v, acc);
-          if (mine) {
-            uint32_t* out = static_cast<uint32_t*>(p.out) + o;
+          for (int b = 0; b < 2; ++b) {
+            if (b == 1 && !two) break;
+            if (mine) {
+              const int left = tl.ncols - c - 64 * b;
+              uint32_t* out = static_cast<uint32_t*>(p.out) + first + (c + 64 * b) * ldc;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < left) out[j * ldc] = w[j];
+              for (int j = 0; j < 32; ++j)
+                if (j < left) out[j * ldc] = v[b][j];
+            }
           }
-        } else {
-          uint32_t h[16];  // columns 2 j (low half) and 2 j + 1
-          if (!empty) tmem_ld_wait();
+          continue;
+        }
+        // columns 2 j (low half) and 2 j + 1 of a chunk in word j
+        if (p.out_type == 1) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) h[j] = pack16(p.out_type, v[2 * j], v[2 * j + 1]);
-          if (!empty) next_columns(t_addr, c, left, v, acc);
-          if (p.wide_rows) {
-            // through shared memory to 16-byte stores: the lane writes its 32 columns as 32 rows of 64
-            // bytes (16-byte pieces xor-swizzled by row pair), then four lanes store a row
+          for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = pack16(1, v[j >> 4][2 * (j & 15)], v[j >> 4][2 * (j & 15) + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = pack16(2, v[j >> 4][2 * (j & 15)], v[j >> 4][2 * (j & 15) + 1]);
+        }
+        if (p.wide_rows) {
+          // through shared memory to 16-byte stores: the lane writes its 32 columns as 32 rows of 64 bytes
+          // (16-byte pieces xor-swizzled by row pair), then four lanes store a row
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b == 1 && !two) break;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const uint32_t a = stage_base + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
-              asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1))))
+              const uint32_t a = stage_base + b * (kGroupStage / 2) + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(static_cast<uint16_t>(v[b][j >> 1] >> (16 * (j & 1))))
                            : "memory");
             }
-            __syncwarp();
-            const int piece = lane & 3;
-            const int mp = m - lane + piece * 8;  // (the extent is a multiple of 8: all of a piece or none)
+          }
+          __syncwarp();
+          const int piece = lane & 3;
+          const int mp = m - lane + piece * 8;  // (the extent is a multiple of 8: all of a piece or none)
+          uint4 d[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = i * 8 + (lane >> 2);
-              uint4 d;
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(d.x), "=r"(d.y), "=r"(d.z), "=r"(d.w)
-                           : "r"(stage_base + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
-                           : "memory");
-              if (row < left && mp < p.M)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o - lane + piece * 8 + row * ldc) = d;
+          for (int i = 0; i < 8; ++i) {
+            const int row = (i & 3) * 8 + (lane >> 2);
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(d[i].x), "=r"(d[i].y), "=r"(d[i].z), "=r"(d[i].w)
+                         : "r"(stage_base + (i >> 2) * (kGroupStage / 2) + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                         : "memory");
+          }
+          if (mp < p.M) {
+            uint16_t* out = static_cast<uint16_t*>(p.out) + first - lane + piece * 8 + (c + (lane >> 2)) * ldc;
+            const int left = tl.ncols - c - (lane >> 2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = (i >> 2) * 64 + (i & 3) * 8;
+              if (row < left) *reinterpret_cast<uint4*>(out + row * ldc) = d[i];
             }
-            __syncwarp();
-          } else if (mine) {
-            uint16_t* out = static_cast<uint16_t*>(p.out) + o;
+          }
+          __syncwarp();
+        } else if (mine) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b == 1 && !two) break;
+            const int left = tl.ncols - c - 64 * b;
+            uint16_t* out = static_cast<uint16_t*>(p.out) + first + (c + 64 * b) * ldc;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < left) out[j * ldc] = static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1)));
+              if (j < left) out[j * ldc] = static_cast<uint16_t>(v[b][j >> 1] >> (16 * (j & 1)));
           }
         }
       }
