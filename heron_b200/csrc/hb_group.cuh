@@ -43,10 +43,9 @@ enum { kFwd = 0, kDx = 1, kDw = 2, kMx = 3 };
 
 constexpr int kMaxGroups = 1024;
 constexpr int kSortedGroups = 224;  // a thread each
-// A producer, MMA, eight epilogue warps, B producer; kDw: the zeros behind a group; kMx: the copies of the
-// scales and their producer
+// A producer, MMA, eight epilogue warps, B producer; kDw: the zeros behind a group; kMx: the scales' producer
 constexpr int kGroupEpi = 8;
-__host__ __device__ constexpr int group_threads(int mode) { return 32 * (3 + kGroupEpi + (mode == kMx ? 2 : (mode == kDw ? 1 : 0))); }
+__host__ __device__ constexpr int group_threads(int mode) { return 32 * (3 + kGroupEpi + (mode == kMx || mode == kDw ? 1 : 0)); }
 constexpr int kGroupStage = 4096;      // epilogue staging of a warp: 2 x 32 columns x 32 16-bit values
 constexpr int kSpan = 128;             // bytes of the reduction axis in a ring stage (TMA swizzle span)
 constexpr int kAtomBytes = 512;        // scales of 128 rows x 128 elements
@@ -196,10 +195,10 @@ __device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, i
 struct GroupBars {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
-  uint64_t sf_full[kMaxStages];  // kMx: the stage's scales are in TMEM; kDw: its edge is zero
+  uint64_t edge[kMaxStages];  // kDw: the stage's edge is zero
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
-  uint64_t drain, sf_drain;
+  uint64_t drain;
   uint64_t red_full, red_empty;  // SPLIT: a share's partial sums are here; are read
   uint32_t tmem_base;
   int abort_flag;
@@ -228,7 +227,7 @@ template <int MODE, int CG, bool SPLIT = false>
 __global__ void __launch_bounds__(group_threads(MODE), 1)
 hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ CUtensorMap tmBw,
-                const GroupParams p) {
+                const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const GroupParams p) {
   constexpr bool A_MN = MODE == kDx || MODE == kDw;
   constexpr bool B_MN = MODE == kDw;
   constexpr int kElems = MODE == kMx ? 256 : 64;
@@ -262,14 +261,13 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), MODE == kDw ? 2 : 1);
-      mbar_init(smem_u32(&bars->sf_full[s]), 1);
+      mbar_init(smem_u32(&bars->edge[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&bars->tmem_full[a]), 1);
       mbar_init(smem_u32(&bars->tmem_empty[a]), kGroupEpi * CG);
     }
     mbar_init(smem_u32(&bars->drain), 1);
-    mbar_init(smem_u32(&bars->sf_drain), 1);
     if (SPLIT) {
       mbar_init(smem_u32(&bars->red_full), ks * 2 * max(4 / ks, 1));  // two warps of each quarter of the lanes in a share
       mbar_init(smem_u32(&bars->red_empty), ks * kGroupEpi);
@@ -309,8 +307,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   // product of 192-row tiles), of 64 otherwise
   auto b_boxes = [&](int nmma, int& box) {
     const int mine = nmma / CG;
+    const int cap = p.BN / CG;  // rows that a stage has room for
     if (B_MN) box = 64;
-    else box = mine <= 48 ? 16 : (4 * mine >= 3 * (p.BN / CG) ? p.BN / CG : 64);
+    else box = mine <= 48 ? 16 : (4 * mine >= 3 * cap || round_up(mine, 64) > cap ? cap : 64);
     return (mine + box - 1) / box;
   };
   auto sf_b_rows = [&](const GroupTile& tl) { return ((tl.c0 & 127) + tl.nmma + 127) >> 7; };
@@ -331,12 +330,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const int nb_sf = MODE == kMx ? sf_b_rows(tl) : 0;
       const int m0 = tl.m0 + static_cast<int>(cta_rank) * kTileM;
       const int mine0 = tl.c0 + static_cast<int>(cta_rank) * (tl.nmma / CG);  // first B row / column
-      const uint8_t* sfa = nullptr;
-      const uint8_t* sfb = nullptr;
-      if (MODE == kMx) {
-        sfa = p.sfa + (static_cast<long long>(tl.e) * p.tiles_m + tl.m0 / kTileM) * kt * kAtomBytes;
-        sfb = p.sfb + (static_cast<long long>(tl.start / 128 + tl.e + tl.c0 / 128)) * kt * kAtomBytes;
-      }
+      // tile rows of the scales
+      const int sf_row_a = tl.e * ((p.M + 127) / 128) + m0 / 128;
+      const int sf_row_b = tl.start / 128 + tl.e + tl.c0 / 128;
       for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
         const uint32_t full_local = smem_u32(&bars->full[stage]);
         const uint32_t full = (CG == 2) ? mapa(full_local, 0) : full_local;
@@ -344,8 +340,10 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           ok = false;
           break;
         }
-        const uint32_t sf_tile = MODE == kMx ? min(2, kt - 2 * kb) * kAtomBytes : 0;
-        if (leader && (part & 1)) mbar_arrive_expect_tx(full_local, tx_ab + (1 + nb_sf) * sf_tile);
+        // (an untiled copy completes in its own CTA: the pair's scales come by tensor map, whole boxes)
+        const uint32_t sf_tile = MODE == kMx && CG == 1 ? min(2, kt - 2 * kb) * kAtomBytes : 0;
+        const uint32_t sf_tx = MODE != kMx ? 0 : (CG == 1 ? (1 + nb_sf) * sf_tile : (1 + sf_rows) * 4 * kAtomBytes);
+        if (leader && (part & 1)) mbar_arrive_expect_tx(full_local, tx_ab + sf_tx);
         const uint32_t dA = sA + stage * a_bytes, dB = sB + stage * b_bytes, dSF = sSF + stage * sf_bytes;
         // first index of this block on the reduction axis (in bytes of packed codes for kMx)
         const int red = MODE == kMx ? kb * kSpan : kb * kElems;
@@ -374,10 +372,15 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           }
         }
         if (MODE == kMx && (part & 4)) {
-          bulk_load(dSF, sfa + static_cast<long long>(kb) * 2 * kAtomBytes, sf_tile, full);
-          for (int b = 0; b < nb_sf; ++b)
-            bulk_load(dSF + (1 + b) * 2 * kAtomBytes, sfb + (static_cast<long long>(b) * kt + 2 * kb) * kAtomBytes,
-                      sf_tile, full);
+          if (CG == 1) {
+            bulk_load(dSF, p.sfa + (static_cast<long long>(sf_row_a) * kt + 2 * kb) * kAtomBytes, sf_tile, full);
+            for (int b = 0; b < nb_sf; ++b)
+              bulk_load(dSF + (1 + b) * 2 * kAtomBytes,
+                        p.sfb + (static_cast<long long>(sf_row_b + b) * kt + 2 * kb) * kAtomBytes, sf_tile, full);
+          } else {
+            tma_load_3d_cg<CG>(dSF, &tmSA, full, kb * 256, sf_row_a, 0);
+            tma_load_3d_cg<CG>(dSF + 2 * kAtomBytes, &tmSB, full, kb * 256, sf_row_b, 0);
+          }
         }
         ++issued;
         if (++stage == p.stages) {
@@ -419,7 +422,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     constexpr uint32_t a_lo_fixed = (A_MN ? chunk16 : 1u) << 16, b_lo_fixed = (B_MN ? chunk16 : 1u) << 16;
     constexpr uint32_t a_step = A_MN ? 16u * kSpan >> 4 : 2u, b_step = B_MN ? 16u * kSpan >> 4 : 2u;
     const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
-    const uint32_t sf_full0 = smem_u32(&bars->sf_full[0]);
+    const uint32_t edge0 = smem_u32(&bars->edge[0]);
     const uint32_t sf_cols = static_cast<uint32_t>(8 * (1 + sf_rows));  // TMEM columns of a stage's scales
     const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
     int at = 0;
@@ -432,9 +435,9 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * p.BN);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tl.nmma >> 3) << 17);
       uint32_t accum = 0u;
+      const int nb_sf = MODE == kMx ? sf_b_rows(tl) : 0;
       for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
         ok = mbar_wait(full0 + 8u * stage, phase, wctx);
-        if (MODE == kMx && ok) ok = mbar_wait(sf_full0 + 8u * stage, phase, wctx);
         if (!ok) break;
         tc_fence_after();
         const uint32_t stA = sA + stage * a_bytes, stB = sB + stage * b_bytes;
@@ -446,7 +449,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (valid < 64) {
             steps = (valid + 15) / 16;
             if (valid & 15) {  // (the rows behind the group's last one are zero when this barrier says so)
-              if (!mbar_wait(sf_full0 + 8u * stage, (edges >> stage) & 1u, wctx)) {
+              if (!mbar_wait(edge0 + 8u * stage, (edges >> stage) & 1u, wctx)) {
                 ok = false;
                 break;
               }
@@ -458,15 +461,31 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           const uint32_t a_lo = ((stA >> 4) & 0x3FFFu) | a_lo_fixed, b_lo = ((stB >> 4) & 0x3FFFu) | b_lo_fixed;
           uint32_t ta = 0, tb = 0;
           if constexpr (MODE == kMx) {
+            // Scales into TMEM, in order before the MMAs of this thread.  A stage has its own columns: they
+            // are written again only after the MMAs that read them have freed the stage.  Columns: A's two
+            // tiles of 128 elements, then per tile of 128 elements B's tile rows side by side (column j
+            // holds rows 32 j ...).  (Copied by another thread, with a barrier between, a stage waits for
+            // the copies' completion: 43.7 us where this takes 39.4 for 4096^3.)
             ta = sf_tmem + stage * sf_cols;
-            tb = ta + 8u + static_cast<uint32_t>((tl.c0 & 127) >> 5);
+            tb = ta + 8u;
+            const uint32_t sf = sSF + stage * sf_bytes;
+#pragma unroll
+            for (int ka = 0; ka < 2; ++ka) {
+              if (2 * ka < steps) {
+                tmem_cp_scales<CG>(ta + 4u * ka, sf + ka * kAtomBytes);
+                tmem_cp_scales<CG>(tb + static_cast<uint32_t>(4 * ka * sf_rows), sf + (2 + ka) * kAtomBytes);
+                if (nb_sf > 1)
+                  tmem_cp_scales<CG>(tb + static_cast<uint32_t>(4 * ka * sf_rows + 4), sf + (4 + ka) * kAtomBytes);
+              }
+            }
+            tb += static_cast<uint32_t>((tl.c0 & 127) >> 5);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (k < steps) {
               const uint64_t ad = desc_hi | (a_lo + a_step * k), bd = desc_hi | (b_lo + b_step * k);
               if constexpr (MODE == kMx)
-                umma_mxf4(d_tmem, ad, bd, idesc | (k & 1 ? (2u << 4) | (2u << 29) : 0u), ta + 4u * (k >> 1),
+                umma_mxf4<CG>(d_tmem, ad, bd, idesc | (k & 1 ? (2u << 4) | (2u << 29) : 0u), ta + 4u * (k >> 1),
                           tb + static_cast<uint32_t>(4 * sf_rows * (k >> 1)), accum);
               else
                 umma_cg<CG, 0>(d_tmem, ad, bd, idesc, accum);
@@ -490,46 +509,6 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     if (!ok) {
       umma_commit_local<CG>(smem_u32(&bars->drain));
       mbar_wait_drain(smem_u32(&bars->drain), 0u);
-    }
-  };
-
-  // kMx: the scales of a stage from shared memory to TMEM, by a thread of its own (see kMx above).  A
-  // stage has its own columns: they are written again only after the MMAs that read them have freed the
-  // stage.  Columns: A's two tiles of 128 elements, then per tile of 128 elements B's tile rows side by
-  // side (column j holds rows 32 j ...).
-  auto copy_scales = [&]() {
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    const uint32_t sf_cols = static_cast<uint32_t>(8 * (1 + sf_rows));
-    const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(p.acc_stages * p.BN);
-    int at = 0;
-    GroupTile tl;
-    for (int i = 0; ok && take(at, i, tl); ++i) {
-      const int nb_sf = sf_b_rows(tl);
-      for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
-        if (!mbar_wait(smem_u32(&bars->full[stage]), phase, wctx)) {
-          ok = false;
-          break;
-        }
-        const uint32_t ta = sf_tmem + stage * sf_cols, tb = ta + 8u;
-        const uint32_t sf = sSF + stage * sf_bytes;
-        const int tiles_k = min(2, (p.R - kb * kElems + 127) / 128);
-        for (int ka = 0; ka < tiles_k; ++ka) {
-          tmem_cp_scales(ta + 4u * ka, sf + ka * kAtomBytes);
-          for (int i = 0; i < nb_sf; ++i)
-            tmem_cp_scales(tb + static_cast<uint32_t>(ka * 4 * sf_rows + 4 * i), sf + ((1 + i) * 2 + ka) * kAtomBytes);
-        }
-        umma_commit(smem_u32(&bars->sf_full[stage]));
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    if (!ok) {
-      umma_commit(smem_u32(&bars->sf_drain));
-      mbar_wait_drain(smem_u32(&bars->sf_drain), 0u);
     }
   };
 
@@ -558,7 +537,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bars->sf_full[stage]));
+          if (lane == 0) mbar_arrive(smem_u32(&bars->edge[stage]));
         }
         // (a stage is refilled only when this warp has passed it too: its waits never fall a turn behind)
         if (lane == 0) mbar_arrive(smem_u32(&bars->empty[stage]));
@@ -583,9 +562,6 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     clear_edges();
     __syncwarp();
   } else if (MODE == kMx && warp == 3 + kGroupEpi) {
-    if (elect_one()) copy_scales();
-    __syncwarp();
-  } else if (MODE == kMx && warp == 4 + kGroupEpi) {
     if (elect_one()) produce(4);
     __syncwarp();
   } else {
@@ -744,16 +720,22 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = pack16(2, v[j >> 4][2 * (j & 15)], v[j >> 4][2 * (j & 15) + 1]);
         }
         if (p.wide_rows) {
-          // through shared memory to 16-byte stores: the lane writes its 32 columns as 32 rows of 64 bytes
-          // (16-byte pieces xor-swizzled by row pair), then four lanes store a row
+          // Through shared memory to 16-byte stores: a chunk as 32 rows (columns) of 64 bytes, 16-byte pieces
+          // xor-swizzled by row pair.  Neighbouring lanes exchange halves first, so that a lane stores the
+          // values of two features of one column (even lanes the even column): 128 bytes a store without a
+          // bank conflict.  The MMA's operands come through the same shared memory, which is what bounds the
+          // 4-bit products (two-byte stores to shared memory took 3 times the cycles there, and two-byte
+          // stores to memory 45 us where 4096^3 takes 39).
+          const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
+          const uint32_t pair_base = stage_base + (lane & 1) * 64 + ((lane >> 1) & 3) * 4;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             if (b == 1 && !two) break;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const uint32_t a = stage_base + b * (kGroupStage / 2) + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
-              asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(static_cast<uint16_t>(v[b][j >> 1] >> (16 * (j & 1))))
-                           : "memory");
+            for (int j = 0; j < 16; ++j) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, v[b][j], 1);
+              const uint32_t a = pair_base + b * (kGroupStage / 2) + j * 128 + (((lane >> 3) ^ (j & 3)) << 4);
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(__byte_perm(v[b][j], other, pick)) : "memory");
             }
           }
           __syncwarp();

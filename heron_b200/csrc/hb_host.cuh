@@ -58,7 +58,8 @@ bool setup_device(Driver* d) {
   if (prop.major != 10) return false;
   d->sm_count = prop.multiProcessorCount;
   // Opt in to the large dynamic shared-memory carve-out for every kernel instantiation.
-  const void* kernels[39] = {
+  const void* kernels[40] = {
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 2>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1, true>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 1, true>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1>),
@@ -398,6 +399,7 @@ struct hb_plan {
   int group_mode;
   hb::GroupParams gp;
   size_t group_zero_bytes;
+  CUtensorMap tmSA, tmSB;  // scales (CTA pairs)
   bool group_rows;  // few rows: the kernels of hb_rows.cuh on rp instead
   hb::RowsParams rp;
   // NCHW operators only: one launch that brings input and filter to NHWC / HWIO first (the conv

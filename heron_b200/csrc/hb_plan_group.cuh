@@ -29,7 +29,7 @@ long long most_tiles(const GroupProblem& g, const hb_knobs& k) {
 }
 
 int group_stage(const GroupProblem& g, int BN, int cg) {
-  if (g.mode == hb::kMx) return hb::group_stage_bytes<hb::kMx, 1>(BN);
+  if (g.mode == hb::kMx) return cg == 2 ? hb::group_stage_bytes<hb::kMx, 2>(BN) : hb::group_stage_bytes<hb::kMx, 1>(BN);
   return cg == 2 ? hb::group_stage_bytes<hb::kFwd, 2>(BN) : hb::group_stage_bytes<hb::kFwd, 1>(BN);
 }
 
@@ -44,7 +44,7 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
   if (in) k = *in; else std::memset(&k, 0, sizeof(k));
   const int avg = g.T / g.E;  // mean rows of a group
   if (k.cta_group == 0)
-    k.cta_group = ((g.mode == hb::kFwd || g.mode == hb::kDx) && avg >= 256 && g.M >= 256 && k.tile_n % 128 == 0) ? 2 : 1;
+    k.cta_group = (g.mode != hb::kDw && avg >= (g.mode == hb::kMx ? 128 : 256) && g.M >= 256 && (k.tile_n == 0 || k.tile_n >= 128)) ? 2 : 1;
   if (k.tile_n == 0) {
     if (g.mode == hb::kDw)
       k.tile_n = g.C > 128 ? 256 : (g.C > 64 ? 128 : 64);
@@ -70,7 +70,9 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
   const int room = kSmemLimit - group_fixed_smem(g.E, k.split_k > 1);
   if (k.stages == 0) {
     k.stages = room / group_stage(g, k.tile_n, k.cta_group);
-    const int most = g.mode == hb::kMx ? (512 - k.tile_n) / (8 * (1 + hb::group_sf_rows(k.tile_n))) : hb::kMaxStages;
+    // (kMx: TMEM columns of the scales beside two accumulators, or one where two leave none)
+    const int sf = 8 * (1 + hb::group_sf_rows(k.tile_n));
+    const int most = g.mode == hb::kMx ? (512 - (2 * k.tile_n + 2 * sf <= 512 ? 2 : 1) * k.tile_n) / sf : hb::kMaxStages;
     if (k.stages > most) k.stages = most;
     if (k.stages > hb::kMaxStages) k.stages = hb::kMaxStages;
     if (k.stages < 1) k.stages = 1;
@@ -84,10 +86,8 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
 
 int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
   if (k.cta_group != 1 && k.cta_group != 2) return HB_ERR_KNOB;
-  if (k.cta_group == 2 && g.mode != hb::kFwd && g.mode != hb::kDx) return HB_ERR_KNOB;
-  // B is fetched in boxes of 64 rows (16 for narrow tiles): a CTA's share of a tile holds whole boxes
-  const int step = k.cta_group == 2 ? 128 : 64;
-  if (k.tile_n < step || k.tile_n > 256 || k.tile_n % step != 0) return HB_ERR_KNOB;
+  if (k.cta_group == 2 && g.mode == hb::kDw) return HB_ERR_KNOB;
+  if (k.tile_n < 64 * k.cta_group || k.tile_n > 256 || k.tile_n % 64 != 0) return HB_ERR_KNOB;
   if (k.stages < 1 || k.stages > hb::kMaxStages) return HB_ERR_KNOB;
   if (k.acc_stages < 1 || k.acc_stages > 2) return HB_ERR_KNOB;
   if (k.max_ctas < 0) return HB_ERR_KNOB;
@@ -114,6 +114,19 @@ bool few_rows(const GroupProblem& g) {
 // Knobs of the tile kernel, given by the caller: then that kernel is meant.
 bool knob_names_tiles(const hb_knobs& k) {
   return k.tile_n || k.split_k || k.stages || k.acc_stages || k.max_ctas || k.cta_group || k.silent_producer;
+}
+
+// Scale tiles (512 bytes, kt to a tile row) as rows of words: boxes of two tiles and `rows` tile rows, dense in
+// shared memory.
+int encode_scales(Driver& d, CUtensorMap* m, const void* ptr, uint64_t kt, uint64_t tile_rows, uint32_t rows) {
+  cuuint64_t dims[3] = {kt * 128, tile_rows, 1};
+  cuuint64_t strides[2] = {kt * hb::kAtomBytes, kt * hb::kAtomBytes * tile_rows};
+  cuuint32_t box[3] = {256, rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = d.tiled(m, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? HB_OK : HB_ERR_LAUNCH;
 }
 
 // A: w (kFwd, kDx, kMx) or x (kDw); B: the token matrix (kDw: dy).
@@ -205,7 +218,13 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
     rc = encode_tiled3(d, &plan->tmA, HB_U8, A, row, M, E, row, row * M, 128, hb::kTileM, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, HB_U8, B, row, T, 1, row, row * T, 128, 64, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB2, HB_U8, B, row, T, 1, row, row * T, 128, 16, 128);
-    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmC, HB_U8, B, row, T, 1, row, row * T, 128, k.tile_n, 128);
+    if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmC, HB_U8, B, row, T, 1, row, row * T, 128, k.tile_n / k.cta_group, 128);
+    if (rc == HB_OK && k.cta_group == 2) {
+      const uint64_t kt = (R + 127) / 128;
+      rc = encode_scales(d, &plan->tmSA, sfa, kt, E * ((M + 127) / 128), 1);
+      const uint64_t rows_b = offsets ? T / 128 + E : (T + 127) / 128;
+      if (rc == HB_OK) rc = encode_scales(d, &plan->tmSB, sfb, kt, rows_b, hb::group_sf_rows(k.tile_n));
+    }
   } else if (dw) {
     rc = encode_tiled3(d, &plan->tmA, g.in, A, M, T, 1, M * 2, M * 2 * T, 64, 64, 128);
     if (rc == HB_OK) rc = encode_tiled3(d, &plan->tmB, g.in, B, C, T, 1, C * 2, C * 2 * T, 64, 64, 128);
@@ -261,7 +280,7 @@ int launch_group(const hb_plan* plan, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG, SPLIT>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->gp);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG, SPLIT>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->tmSA, plan->tmSB, plan->gp);
   return e == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
@@ -298,7 +317,7 @@ int run_group(const hb_plan* plan, cudaStream_t stream) {
     case hb::kFwd: return pair ? launch_group<hb::kFwd, 2>(plan, stream) : launch_group<hb::kFwd, 1>(plan, stream);
     case hb::kDx: return pair ? launch_group<hb::kDx, 2>(plan, stream) : launch_group<hb::kDx, 1>(plan, stream);
     case hb::kDw: return launch_group<hb::kDw, 1>(plan, stream);
-    default: return launch_group<hb::kMx, 1>(plan, stream);
+    default: return pair ? launch_group<hb::kMx, 2>(plan, stream) : launch_group<hb::kMx, 1>(plan, stream);
   }
 }
 

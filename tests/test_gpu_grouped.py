@@ -88,7 +88,7 @@ def test_forward_takes_any_output_width(K, n):
 
 
 @pytest.mark.parametrize("knobs", [dict(tile_n=64), dict(tile_n=128), dict(tile_n=192), dict(tile_n=256),
-                                   dict(tile_n=128, cta_group=2), dict(tile_n=256, cta_group=2),
+                                   dict(tile_n=128, cta_group=2), dict(tile_n=256, cta_group=2), dict(tile_n=192, cta_group=2),
                                    dict(stages=1), dict(acc_stages=1), dict(max_ctas=2), dict(max_ctas=3, stages=2)])
 def test_knobs_do_not_change_the_product(K, knobs):
     c = [300, 0, 1, 97, 514]

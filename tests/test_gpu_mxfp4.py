@@ -138,7 +138,9 @@ def test_product(K, M, N, k, out_dtype):
 
 
 @pytest.mark.parametrize("knobs", [dict(tile_n=64), dict(tile_n=128), dict(tile_n=192), dict(tile_n=256),
-                                   dict(stages=1), dict(acc_stages=1), dict(max_ctas=2), dict(tile_n=192, max_ctas=1)])
+                                   dict(stages=1), dict(acc_stages=1), dict(max_ctas=2), dict(tile_n=192, max_ctas=1),
+                                   dict(tile_n=128, cta_group=2), dict(tile_n=192, cta_group=2), dict(tile_n=256, cta_group=2),
+                                   dict(tile_n=192, cta_group=2, stages=1), dict(tile_n=192, cta_group=2, max_ctas=2)])
 def test_product_knobs(K, knobs):
     product(K, 700, 300, 800, 11, torch.float32, knobs)
     product(K, 130, 200, 160, 12, torch.float32, knobs)
@@ -205,7 +207,8 @@ def test_grouped_product(K, counts, lead, tail, k, n):
     K.dequantize_mxfp4(xc, xs, offsets=offsets, out=xv)
     wv = K.dequantize_mxfp4(wc, ws)
     want, mag, own = grouped(xv, wv, off)
-    for knobs in (None, dict(tile_n=64), dict(tile_n=192), dict(tile_n=256)):
+    for knobs in (None, dict(tile_n=64), dict(tile_n=192), dict(tile_n=256), dict(tile_n=192, cta_group=2),
+                  dict(tile_n=256, cta_group=2)):
         out = torch.full((T, n), 7.0, device="cuda")
         K.grouped_gemm_mxfp4(xc, xs, wc, ws, offsets, out=out, knobs=knobs)
         assert_product(out[own], want[own], mag[own], k, str(knobs))
