@@ -276,6 +276,12 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
+    prefetch_tmap(&tmB16);
+    prefetch_tmap(&tmBw);
+    if (MODE == kMx && CG == 2) {
+      prefetch_tmap(&tmSA);
+      prefetch_tmap(&tmSB);
+    }
   }
   if (warp == 1) tmem_alloc_cg<CG>(smem_u32(&bars->tmem_base), static_cast<uint32_t>(p.tmem_cols));
   tc_fence_before();
@@ -679,97 +685,116 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
         continue;
       }
-      // two of this warp's chunks of 32 columns at a time, 64 columns apart: the latencies of one (TMEM,
-      // shared memory) pass under the other's
-      for (int c = half * 32; c < tl.ncols; c += 128) {
-        const bool two = c + 64 < tl.ncols;
-        uint32_t v[2][32];
-        if (empty) {
+      // this warp's chunks of 32 columns start at half * 32 + 64 i, i < 4
+      // (the row pitch is opaque here: its multiples, computed once for all tiles, would take 64 registers
+      // and spill)
+      long long ldc = p.ldc;
+      asm volatile("" : "+l"(ldc));
+      if (p.out_type == 0) {
+        for (int c = half * 32; c < tl.ncols; c += 64) {
+          uint32_t v[32];
+          if (empty) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[0][j] = v[1][j] = 0u;
-        } else {
-          tmem_ld_32x32(t_addr + c, v[0]);
-          if (two) tmem_ld_32x32(t_addr + c + 64, v[1]);
-          tmem_ld_wait();
-          if (c + 128 >= tl.ncols) hand_back(acc);  // last read of this accumulator
-        }
-        // (opaque here: multiples of the row pitch, computed once for all tiles, would take 64 registers
-        // and spill)
-        long long ldc = p.ldc;
-        asm volatile("" : "+l"(ldc));
-        if (p.out_type == 0) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b == 1 && !two) break;
-            if (mine) {
-              const int left = tl.ncols - c - 64 * b;
-              uint32_t* out = static_cast<uint32_t*>(p.out) + first + (c + 64 * b) * ldc;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < left) out[j * ldc] = v[b][j];
-            }
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
+          } else {
+            tmem_ld_32x32(t_addr + c, v);
+            tmem_ld_wait();
+            if (c + 64 >= tl.ncols) hand_back(acc);  // last read of this accumulator
           }
-          continue;
-        }
-        // columns 2 j (low half) and 2 j + 1 of a chunk in word j
-        if (p.out_type == 1) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = pack16(1, v[j >> 4][2 * (j & 15)], v[j >> 4][2 * (j & 15) + 1]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = pack16(2, v[j >> 4][2 * (j & 15)], v[j >> 4][2 * (j & 15) + 1]);
-        }
-        if (p.wide_rows) {
-          // Through shared memory to 16-byte stores: a chunk as 32 rows (columns) of 64 bytes, 16-byte pieces
-          // xor-swizzled by row pair.  Neighbouring lanes exchange halves first, so that a lane stores the
-          // values of two features of one column (even lanes the even column): 128 bytes a store without a
-          // bank conflict.  The MMA's operands come through the same shared memory, which is what bounds the
-          // 4-bit products (two-byte stores to shared memory took 3 times the cycles there, and two-byte
-          // stores to memory 45 us where 4096^3 takes 39).
-          const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
-          const uint32_t pair_base = stage_base + (lane & 1) * 64 + ((lane >> 1) & 3) * 4;
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b == 1 && !two) break;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const uint32_t other = __shfl_xor_sync(0xffffffffu, v[b][j], 1);
-              const uint32_t a = pair_base + b * (kGroupStage / 2) + j * 128 + (((lane >> 3) ^ (j & 3)) << 4);
-              asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(__byte_perm(v[b][j], other, pick)) : "memory");
-            }
-          }
-          __syncwarp();
-          const int piece = lane & 3;
-          const int mp = m - lane + piece * 8;  // (the extent is a multiple of 8: all of a piece or none)
-          uint4 d[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int row = (i & 3) * 8 + (lane >> 2);
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(d[i].x), "=r"(d[i].y), "=r"(d[i].z), "=r"(d[i].w)
-                         : "r"(stage_base + (i >> 2) * (kGroupStage / 2) + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
-                         : "memory");
-          }
-          if (mp < p.M) {
-            uint16_t* out = static_cast<uint16_t*>(p.out) + first - lane + piece * 8 + (c + (lane >> 2)) * ldc;
-            const int left = tl.ncols - c - (lane >> 2);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = (i >> 2) * 64 + (i & 3) * 8;
-              if (row < left) *reinterpret_cast<uint4*>(out + row * ldc) = d[i];
-            }
-          }
-          __syncwarp();
-        } else if (mine) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b == 1 && !two) break;
-            const int left = tl.ncols - c - 64 * b;
-            uint16_t* out = static_cast<uint16_t*>(p.out) + first + (c + 64 * b) * ldc;
+          if (mine) {
+            uint32_t* out = static_cast<uint32_t*>(p.out) + first + c * ldc;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < left) out[j * ldc] = static_cast<uint16_t>(v[b][j >> 1] >> (16 * (j & 1)));
+              if (j < tl.ncols - c) out[j * ldc] = v[j];
           }
+        }
+      } else {
+        // All of them to registers, rounded and in pairs (columns 2 j and 2 j + 1 of a chunk in word j), and the
+        // accumulator back, before anything is stored: a tile of 256 columns has no second accumulator beside
+        // the scales, and the MMA warp would wait for the stores (4096^3 in 4 bits 37.8 us, 34.6 so).
+        uint32_t h[4][16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = half * 32 + 64 * i;
+          if (c >= tl.ncols) break;
+          uint32_t v[32];
+          if (empty) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
+          } else {
+            tmem_ld_32x32(t_addr + c, v);
+            tmem_ld_wait();
+          }
+          if (p.out_type == 1) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) h[i][j] = pack16(1, v[2 * j], v[2 * j + 1]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) h[i][j] = pack16(2, v[2 * j], v[2 * j + 1]);
+          }
+        }
+        if (!empty) hand_back(acc);
+        // Through shared memory to 16-byte stores, two chunks at a time: a chunk as 32 rows (columns) of 64
+        // bytes, 16-byte pieces xor-swizzled by row pair.  Neighbouring lanes exchange halves first, so that
+        // a lane stores the values of two features of one column (even lanes the even column): 128 bytes a
+        // store without a bank conflict.  The MMA's operands come through the same shared memory.  (Two-byte
+        // stores to shared memory: 39.4 us where this takes 37.3; two-byte stores to memory: 45.)
+        const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
+        const uint32_t pair_base = stage_base + (lane & 1) * 64 + ((lane >> 1) & 3) * 4;
+        const int piece = lane & 3;
+        const int mp = m - lane + piece * 8;  // (the extent is a multiple of 8: all of a piece or none)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const int c = half * 32 + 64 * i;
+          if (c >= tl.ncols) break;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b == 1 && c + 64 >= tl.ncols) break;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, h[i + b][j], 1);
+              const uint32_t a = pair_base + b * (kGroupStage / 2) + j * 128 + (((lane >> 3) ^ (j & 3)) << 4);
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(__byte_perm(h[i + b][j], other, pick)) : "memory");
+            }
+          }
+          __syncwarp();
+          if (p.wide_rows) {
+            uint4 d[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int row = (u & 3) * 8 + (lane >> 2);
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(d[u].x), "=r"(d[u].y), "=r"(d[u].z), "=r"(d[u].w)
+                           : "r"(stage_base + (u >> 2) * (kGroupStage / 2) + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                           : "memory");
+            }
+            if (mp < p.M) {
+              uint16_t* out = static_cast<uint16_t*>(p.out) + first - lane + piece * 8 + (c + (lane >> 2)) * ldc;
+              const int left = tl.ncols - c - (lane >> 2);
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const int row = (u >> 2) * 64 + (u & 3) * 8;
+                if (row < left) *reinterpret_cast<uint4*>(out + row * ldc) = d[u];
+              }
+            }
+          } else {
+            // rows of any length and alignment: a value a lane.  (Rolled: 32 stores a chunk written out, straight
+            // from the registers, cost 1003 rows of 1001 features 4250 cycles a tile, mostly instruction fetch.)
+            for (int b = 0; b < 2; ++b) {
+              const int rows = min(tl.ncols - c - 64 * b, 32);
+              uint16_t* out = static_cast<uint16_t*>(p.out) + first + (c + 64 * b) * ldc;
+#pragma unroll 4
+              for (int row = 0; row < rows; ++row, out += ldc) {
+                uint16_t d;
+                asm volatile("ld.shared.u16 %0, [%1];"
+                             : "=h"(d)
+                             : "r"(stage_base + b * (kGroupStage / 2) + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) << 4) + (lane & 7) * 2)
+                             : "memory");
+                if (mine) *out = d;
+              }
+            }
+          }
+          __syncwarp();
         }
       }
       if (!empty && ++acc == p.acc_stages) {

@@ -49,7 +49,7 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
     if (g.mode == hb::kDw)
       k.tile_n = g.C > 128 ? 256 : (g.C > 64 ? 128 : 64);
     else if (g.mode == hb::kMx)
-      k.tile_n = avg > 128 ? 192 : (avg > 48 ? 128 : 64);
+      k.tile_n = k.cta_group == 2 ? 256 : (avg > 128 ? 192 : (avg > 48 ? 128 : 64));
     else
       k.tile_n = k.cta_group == 2 || avg > 96 ? 256 : (avg > 48 ? 128 : 64);
   }
