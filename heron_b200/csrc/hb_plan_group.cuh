@@ -43,12 +43,20 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
   hb_knobs k;
   if (in) k = *in; else std::memset(&k, 0, sizeof(k));
   const int avg = g.T / g.E;  // mean rows of a group
+  // CTA pairs: half of B to each CTA.  Measured, single CTAs against pairs, both with their best tile, in a loop
+  // of half a second: 8192 rows, 32 groups of 2048 x 2048 bf16 94 / 84 us; dx of 16 groups of 512 rows 47.7 / 42.1;
+  // MXFP4 4096^3 43.7 / 39.5, 187 rows a group 31.8 / 29.8.  dw by pairs (its edge rows cleared in both CTAs)
+  // was level, 49.4 / 49.2, and is not built.
   if (k.cta_group == 0)
     k.cta_group = (g.mode != hb::kDw && avg >= (g.mode == hb::kMx ? 128 : 256) && g.M >= 256 && (k.tile_n == 0 || k.tile_n >= 128)) ? 2 : 1;
   if (k.tile_n == 0) {
     if (g.mode == hb::kDw)
-      k.tile_n = g.C > 128 ? 256 : (g.C > 64 ? 128 : 64);
+      // (up to 64 rows a group a tile is one block and its time the epilogue's, which narrower tiles spread
+      // better: 777 rows, 20 groups of 328 x 520 8.9 us with 128 columns, 9.7 with 256; 512 rows a group 57 / 48)
+      k.tile_n = g.C > 128 && avg > 64 ? 256 : (g.C > 64 ? 128 : 64);
     else if (g.mode == hb::kMx)
+      // (two accumulators and the scales fit TMEM beside 192 columns; pairs take 256 and one accumulator: 4096^3
+      // 37.5 us with 192, 34.6 with 256; single CTAs 37.3 with 192, 46 with 128)
       k.tile_n = k.cta_group == 2 ? 256 : (avg > 128 ? 192 : (avg > 48 ? 128 : 64));
     else
       k.tile_n = k.cta_group == 2 || avg > 96 ? 256 : (avg > 48 ? 128 : 64);
@@ -165,8 +173,7 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
     r.out_type = out_type_of(g.out);
     r.w_matrix_sf = mx ? (g.M + 127LL) / 128 * ((g.R + 127LL) / 128) * hb::kAtomBytes : 0;
     plan->group_rows = true;
-    plan->group_mode = mx ? hb::kMx : (g.in == HB_F16 ? 1 : 2);
-    plan->knobs = k;
+    plan->group_mode = mx ? hb::kMx : (g.in == HB_F16 ? 1 : 2);  // (no knobs: they are the tile kernel's)
     // (4-bit: 16 features to a block within a tile of 128)
     plan->grid = mx ? (g.M + 127) / 128 * 8 : (g.M + hb::kRowsFeatures - 1) / hb::kRowsFeatures;
     return HB_OK;

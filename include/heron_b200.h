@@ -319,7 +319,10 @@ int hb_conv2d_nhwc_packed_noalloc(const void* in, const void* w_packed, void* ou
  * fixed order, one rounding at the end.  Dense row-major buffers; K % 8 == 0, for the gradients
  * also N % 8 == 0; 1 <= E <= 1024; T >= 0 (T = 0: only the weight gradient is written).
  * Knobs used: tile_n (64, 128, 192, 256: the widest tile of a group's rows; of N in dw), stages,
- * acc_stages, cta_group (2: not dw, tile_n 128 or 256), max_ctas, silent_producer; the rest is ignored.
+ * acc_stages, cta_group (2: not dw, tile_n at least 128), split_k (1, 2, 4, 8: CTAs of a cluster that share
+ * the reduction of a tile; forward products with tile_n 64 and cta_group 1), max_ctas, silent_producer; the
+ * rest is ignored.  A call that sets none of these may run on a kernel without tiles where there are
+ * few rows (hb_plan_knobs then reports zeros).
  */
 int hb_grouped_gemm(const void* x, const void* w, void* out, const int* offsets, int T, int K, int N,
                     int E, hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, void* stream);
@@ -351,7 +354,7 @@ int hb_grouped_gemm_dw(const void* dy, const void* x, void* dw, const int* offse
  * fp32 accumulation, out HB_F32, HB_F16 or HB_BF16.  hb_grouped_gemm_mxfp4: hb_grouped_gemm with x
  * quantised by groups and w (E,N,K) quantised as a batch.  Scales as written above, pad bytes
  * included (a pad byte of 255 would turn its row into NaN).  Sizes, knobs and offsets as for
- * hb_grouped_gemm, with K % 32 == 0 and cta_group 1.  No entry point here needs a workspace.
+ * hb_grouped_gemm, with K % 32 == 0.  No entry point here needs a workspace.
  */
 size_t hb_mxfp4_scale_bytes(int batch, int rows, int K, int groups);
 int hb_quantize_mxfp4(const void* x, void* codes, void* scales, const int* offsets, int batch, int rows,

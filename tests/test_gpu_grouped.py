@@ -250,8 +250,8 @@ def test_a_silent_producer_ends_in_a_status(K):
     for fn, args in ((K.grouped_gemm, (x, w)), (K.grouped_gemm_dx, (dy, w)), (K.grouped_gemm_dw, (dy, x))):
         fn(*args, offsets, knobs=dict(silent_producer=1))
         assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
-    fn = K.grouped_gemm
-    fn(x, w, offsets, knobs=dict(silent_producer=1, cta_group=2, tile_n=128))
-    assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
+    for knobs in (dict(silent_producer=1, cta_group=2, tile_n=128), dict(silent_producer=1, tile_n=64, split_k=4)):
+        K.grouped_gemm(x, w, offsets, knobs=knobs)
+        assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
     want, mag, _ = grouped(x, w, off)
     assert_product(K.grouped_gemm(x, w, offsets), want, mag, 128)

@@ -247,8 +247,10 @@ def test_no_rows(K):
 def test_a_silent_producer_ends_in_a_status(K):
     from heron_b200 import _lib
     a, b = K.quantize_mxfp4(randn(1, 64, 256)), K.quantize_mxfp4(randn(2, 128, 256))
-    K.gemm_mxfp4(*a, *b, knobs=dict(silent_producer=1))
-    assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
+    for knobs in (dict(silent_producer=1), dict(silent_producer=1, cta_group=2, tile_n=192),
+                  dict(silent_producer=1, tile_n=64, split_k=2)):
+        K.gemm_mxfp4(*a, *b, knobs=knobs)
+        assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
     want = K.dequantize_mxfp4(*a).double() @ K.dequantize_mxfp4(*b).double().T
     mag = K.dequantize_mxfp4(*a).double().abs() @ K.dequantize_mxfp4(*b).double().abs().T
     assert_product(K.gemm_mxfp4(*a, *b), want, mag, 256)
