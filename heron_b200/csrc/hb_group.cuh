@@ -13,9 +13,9 @@
 // always the contiguous axis of the output (a feature), never the ragged one: a tile's columns are
 // tokens, and the width of an MMA is chosen per tile in steps of 16 (N of tcgen05.mma), so a group of
 // five rows costs a 128 x 16 product and not a 128 x 128 one.  With the roles the other way round a
-// group's last tile would always be computed 128 rows high.  The epilogue thread of lane m then
-// stores its columns one output row at a time: a warp's 32 lanes write 64 or 128 consecutive bytes,
-// whole sectors whatever the extents, so no output extent has an alignment rule.
+// group's last tile would always be computed 128 rows high.  The epilogue stores output rows: 32 lanes of
+// fp32 are 128 consecutive bytes; 16-bit values go through shared memory to 16-byte pieces, or one by one
+// where a row is no multiple of 16 bytes, so no output extent has an alignment rule.
 //
 //   mode   A (M axis)                     B (columns)              reduction
 //   kFwd   w, K-major                     x, K-major               K
@@ -31,7 +31,18 @@
 // Tiles are listed on the device: every CTA reads the offsets, keeps the groups that have rows (all
 // of them in kDw) with a running count of tiles in shared memory, and walks tiles blockIdx.x,
 // blockIdx.x + gridDim.x, ...  A group's rows are cut into equal tiles, not full ones and a rest, so
-// that the tiles of a wave cost about the same.  Offsets are clamped to [0, T] and a group whose end
+// that the tiles of a wave cost about the same.
+//
+// A CTA pair (CG = 2) shares tiles of 256 features as in hb_umma_kernel; in kMx each CTA brings the scales of its
+// own features and of all the tile's rows.  SPLIT: the 2, 4 or 8 CTAs of a cluster share a tile's reduction
+// and join their sums through distributed shared memory, in the order of the shares.
+//
+// What bounds it (B200, times in loops of some 10 ms; sustained loops are 15 % slower): 8192 rows over 32 experts of
+// 2048 x 2048 bf16 71 us, 335 MB of traffic at 4.7 TB/s and 57 % of the tensor cycles; dx of 8192 rows, 16 groups of
+// 2048 x 1024 36 us; dw of the same 41 us, where operands into and out of shared memory (48 KB a block each way)
+// take longer than the MMAs; 4096^3 in 4 bits 34.6 us, where a block's scale copies and MMAs take their issuing
+// thread about as long (460 cycles) as the tensor core (512).
+// Offsets are clamped to [0, T] and a group whose end
 // lies before its start counts as empty: wrong offsets give wrong rows, never an access out of range.
 #pragma once
 #include "hb_kernel.cuh"
@@ -56,7 +67,7 @@ struct GroupParams {
   int M;                // extent of the M axis (the output's contiguous extent)
   int C;                // kDw: extent of the column axis; otherwise unused (columns are a group's rows)
   int R;                // extent of the reduction axis; kDw: unused (a group's rows)
-  int BN;               // widest tile, multiple of 32 (64 in kDw and kMx)
+  int BN;               // widest tile, a multiple of 64
   int stages, acc_stages, tmem_cols, tiles_m;
   int out_type;         // 0: fp32, 1: fp16, 2: bf16
   int wide_rows;        // 16-bit output whose rows are multiples of 16 bytes
@@ -163,30 +174,34 @@ __device__ __forceinline__ int group_list(const GroupParams& p, GroupEntry* g, i
   }
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int kept = 0, sum = 0;
+    int kept = 0;
+    // (in 64 bits and cut at 2^30, which no ascending offsets reach: a row in many groups at once must not make
+    // the counts wrap and a walker run past the list)
+    long long sum = 0;
+    constexpr long long kMost = 1LL << 30;
     for (int base = 0; base < p.E; base += 32) {
       const int e = base + lane;
       const GroupEntry in = e < p.E ? g[e] : GroupEntry{0, 0, 0, 0};
       const int n = in.n;
       const int cols = MODE == kDw ? (e < p.E ? p.C : 0) : n;
-      int tiles = (cols + p.BN - 1) / p.BN * p.tiles_m;
+      const int tiles = (cols + p.BN - 1) / p.BN * p.tiles_m;
       const uint32_t has = __ballot_sync(0xffffffffu, tiles > 0);
-      int incl = tiles;
+      long long incl = tiles;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        const long long v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
       }
       // (every lane holds its group in registers: the entries written below are at or before these)
       if (tiles > 0) {
         const int slot = kept + __popc(has & ((1u << lane) - 1u));
-        g[slot] = GroupEntry{in.e, in.start, n, sum + incl};
+        g[slot] = GroupEntry{in.e, in.start, n, static_cast<int>(min(sum + incl, kMost))};
       }
       __syncwarp();
       kept += __popc(has);
       sum += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) *total = sum;
+    if (lane == 0) *total = static_cast<int>(min(sum, kMost));
   }
   __syncthreads();
   return *total;

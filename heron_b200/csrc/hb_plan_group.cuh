@@ -113,7 +113,8 @@ int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
 // million 6.9 / 9.3 us (one row, 4096 x 4096) and 7.0 / 7.1 (four rows to four experts of 2048 x 2048), twice as
 // many 10.2 / 7.4; and a long reduction over few features is one for the cluster (1024 x 16384 13 / 8.4).
 bool few_rows(const GroupProblem& g) {
-  if (g.mode == hb::kFwd) return g.T <= (g.E > 8 ? g.E : 8);
+  // (at most 64 rows: all of them in one group are then eight passes over its weights)
+  if (g.mode == hb::kFwd) return g.T <= (g.E > 64 ? 64 : (g.E > 8 ? g.E : 8));
   if (g.mode != hb::kMx || g.T > 64 || g.R > 8192) return false;
   const long long passes = g.E == 1 ? (g.T + 7) / 8 : g.T;
   return passes * g.M * g.R <= (1LL << 24);

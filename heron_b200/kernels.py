@@ -611,6 +611,12 @@ def _ptrs(*tensors):
     return ptrs, _raw_stream(dev)
 
 
+def _fits(sizes):
+    """The library's sizes are ints; a larger one would arrive cut to 32 bits."""
+    if max(sizes) > 0x7fffffff:
+        raise _lib.HeronB200Error(_lib.HB_ERR_SHAPE, "sizes %s" % (sizes,))
+
+
 def _groups(offsets, groups=None):
     n = offsets.numel() - 1
     if offsets.dim() != 1 or n < 1 or (groups is not None and n != groups):
@@ -656,6 +662,7 @@ def _grouped_args(kind, first, second, offsets, out, out_dtype):
 
 
 def _run(kind, tensors, sizes, knobs, out):
+    _fits(sizes)
     ptrs, stream = _ptrs(*tensors)
     rc = getattr(_lib.load(), kind)(*ptrs, *sizes, _knobs(knobs), stream)
     if rc:
@@ -664,6 +671,7 @@ def _run(kind, tensors, sizes, knobs, out):
 
 
 def _plan(kind, tensors, sizes, knobs, out):
+    _fits(sizes)
     h = ctypes.c_void_p()
     name = kind.replace("hb_", "hb_plan_", 1)
     _lib.check(getattr(_lib.load(), name)(ctypes.byref(h), *_ptrs(*tensors)[0], *sizes, _knobs(knobs)), name)
@@ -725,6 +733,7 @@ def plan_grouped_gemm_dw(dy, x, offsets, out=None, out_dtype=None, knobs=None):
 def mxfp4_scale_bytes(rows, K, groups=0):
     """Bytes of the scale array of a quantised (rows, K) matrix (include/heron_b200.h has the layout);
     `groups`: of one whose rows are grouped by offsets."""
+    _fits((rows, K, groups))
     n = _lib.load().hb_mxfp4_scale_bytes(1, rows, K, groups)
     if n == 0 and (rows > 0 or groups > 0 or K <= 0 or K % 32):
         raise _lib.HeronB200Error(_lib.HB_ERR_SHAPE, "mxfp4_scale_bytes")
@@ -747,6 +756,7 @@ def _mx_shape(x, K, offsets, what):
 
 
 def _run_mx(kind, tensors, offsets, sizes, code):
+    _fits(sizes)
     if offsets is None:
         ptrs, stream = _ptrs(*tensors)
         ptrs.append(None)

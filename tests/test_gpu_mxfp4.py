@@ -244,6 +244,22 @@ def test_no_rows(K):
     assert K.dequantize_mxfp4(xc, xs).shape == (0, 64)
 
 
+def test_two_streams_at_once(K):
+    """No call keeps anything between calls: the same operands on two streams, outputs of their own."""
+    x, w = randn(1, 300, 512, dtype=torch.bfloat16), randn(2, 260, 512, dtype=torch.bfloat16)
+    wq = K.quantize_mxfp4(w)
+    want = K.gemm_mxfp4(*K.quantize_mxfp4(x), *wq)
+    got, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(K.gemm_mxfp4(*K.quantize_mxfp4(x), *wq))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+
+
 def test_a_silent_producer_ends_in_a_status(K):
     from heron_b200 import _lib
     a, b = K.quantize_mxfp4(randn(1, 64, 256)), K.quantize_mxfp4(randn(2, 128, 256))

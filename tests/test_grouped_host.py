@@ -175,6 +175,21 @@ def test_python_refusals(hb_lib):
         K.gemm_mxfp4(c, s, c, s)
 
 
+def test_sizes_beyond_32_bits_are_refused(hb_lib):
+    """Tensors without memory stand in: the refusal comes before any address is looked at."""
+    from heron_b200 import kernels as K
+    from heron_b200._lib import HeronB200Error
+    for n in (2 ** 31, 2 ** 32 + 64):
+        x = torch.empty(n, 8, dtype=torch.float16, device="meta")
+        w, off = torch.empty(2, 8, 8, dtype=torch.float16, device="meta"), torch.empty(3, dtype=torch.int32, device="meta")
+        with pytest.raises(HeronB200Error):
+            K.grouped_gemm(x, w, off)
+        with pytest.raises(HeronB200Error):
+            K.quantize_mxfp4(torch.empty(n, 32, device="meta"))
+        with pytest.raises(HeronB200Error):
+            K.mxfp4_scale_bytes(n, 32)
+
+
 def test_the_definition_of_the_format():
     """The oracle itself, on values whose codes are known."""
     x = torch.zeros(1, 32)
