@@ -212,9 +212,6 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   int units = d.sm_count / together;
   if (k.max_ctas > 0 && k.max_ctas / together < units) units = k.max_ctas / together;
   if (units < 1) units = 1;
-  // (with fewer rows a group than the narrowest tiles hold all tiles cost the same; the sort takes about 1 us,
-  // which few tiles do not earn back: 777 rows in 20 groups 6.8 us without, 8.1 us with it)
-  p.sorted = tiles > 3LL * units && g.E > 1 && g.E <= hb::kSortedGroups && g.T / g.E >= 32;
   plan->grid = static_cast<int>(tiles < units ? tiles : units) * together;
   p.ksplit = k.split_k;
   plan->smem = group_fixed_smem(g.E, k.split_k > 1) + k.stages * group_stage(g, k.tile_n, k.cta_group);
