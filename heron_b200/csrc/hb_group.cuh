@@ -55,10 +55,15 @@ namespace hb {
 enum { kFwd = 0, kDx = 1, kDw = 2, kMx = 3 };
 
 constexpr int kMaxGroups = 1024;
-// A producer, MMA, eight epilogue warps, B producer; kDw: the zeros behind a group; kMx: the scales' producer
-constexpr int kGroupEpi = 8;
-__host__ __device__ constexpr int group_threads(int mode) { return 32 * (3 + kGroupEpi + (mode == kMx || mode == kDw ? 1 : 0)); }
-constexpr int kGroupStage = 4096;      // epilogue staging of a warp: 2 x 32 columns x 32 16-bit values
+// A producer, MMA, the epilogue warps, B producer; kDw: the zeros behind a group; kMx: the scales' producer.
+// Eight epilogue warps, two to each quarter of the TMEM lanes (with four the weight gradient waited for its
+// accumulators); four in the narrow form, of which two CTAs share an SM.
+__host__ __device__ constexpr int group_epi(bool narrow) { return narrow ? 4 : 8; }
+__host__ __device__ constexpr int group_threads(int mode, bool narrow) {
+  return 32 * (3 + group_epi(narrow) + (mode == kMx || mode == kDw ? 1 : 0));
+}
+// epilogue staging of a warp: 32 columns x 32 16-bit values, twice in the wide form
+__host__ __device__ constexpr int group_staging(bool narrow) { return narrow ? 2048 : 4096; }
 constexpr int kSpan = 128;             // bytes of the reduction axis in a ring stage (TMA swizzle span)
 constexpr int kAtomBytes = 512;        // scales of 128 rows x 128 elements
 
@@ -212,17 +217,19 @@ __device__ __forceinline__ uint32_t pack16(int out_type, uint32_t a, uint32_t b)
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int MODE, int CG, bool SPLIT = false>
-__global__ void __launch_bounds__(group_threads(MODE), 1)
+template <int MODE, int CG, bool SPLIT = false, bool NARROW = false>
+__global__ void __launch_bounds__(group_threads(MODE, NARROW), NARROW ? 2 : 1)
 hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ CUtensorMap tmBw,
                 const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const GroupParams p) {
   constexpr bool A_MN = MODE == kDx || MODE == kDw;
   constexpr bool B_MN = MODE == kDw;
   constexpr int kElems = MODE == kMx ? 256 : 64;
+  constexpr int kGroupEpi = group_epi(NARROW), kGroupStage = group_staging(NARROW);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  static_assert(!NARROW || (CG == 1 && !SPLIT && MODE != kDw), "the narrow form is one of single CTAs");
   static_assert(!SPLIT || (CG == 1 && (MODE == kFwd || MODE == kMx)), "the joined form is that of the forward products");
   const uint32_t cta_rank = (CG == 2) ? cluster_ctarank() : 0u;
   const bool leader = cta_rank == 0u;
@@ -556,10 +563,10 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     if (elect_one()) produce(4);
     __syncwarp();
   } else {
-    // eight warps, two to each quarter of the TMEM lanes, which take its chunks of 32 columns in turn (with
-    // four the weight gradient waited for its accumulators)
+    // this warp's quarter of the TMEM lanes; of two warps of a quarter each takes every second chunk of 32 columns
+    constexpr int kStride = NARROW ? 32 : 64, kChunks = NARROW ? 2 : 4, kAtOnce = NARROW ? 1 : 2;
     const int q = warp & 3;
-    const int half = warp >= 6;
+    const int half = NARROW ? 0 : warp >= 6;
     const uint32_t stage_base = sEpi + (warp - 2) * kGroupStage;
     // gives an accumulator back to the MMA warp
     auto hand_back = [&](int acc) {
@@ -670,13 +677,13 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
         continue;
       }
-      // this warp's chunks of 32 columns start at half * 32 + 64 i, i < 4
+      // this warp's chunks of 32 columns start at half * 32 + kStride i, i < kChunks
       // (the row pitch is opaque here: its multiples, computed once for all tiles, would take 64 registers
       // and spill)
       long long ldc = p.ldc;
       asm volatile("" : "+l"(ldc));
       if (p.out_type == 0) {
-        for (int c = half * 32; c < tl.ncols; c += 64) {
+        for (int c = half * 32; c < tl.ncols; c += kStride) {
           uint32_t v[32];
           if (empty) {
 #pragma unroll
@@ -684,7 +691,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           } else {
             tmem_ld_32x32(t_addr + c, v);
             tmem_ld_wait();
-            if (c + 64 >= tl.ncols) hand_back(acc);  // last read of this accumulator
+            if (c + kStride >= tl.ncols) hand_back(acc);  // last read of this accumulator
           }
           if (mine) {
             uint32_t* out = static_cast<uint32_t*>(p.out) + first + c * ldc;
@@ -697,10 +704,10 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // All of them to registers, rounded and in pairs (columns 2 j and 2 j + 1 of a chunk in word j), and the
         // accumulator back, before anything is stored: a tile of 256 columns has no second accumulator beside
         // the scales, and the MMA warp would wait for the stores (4096^3 in 4 bits 37.8 us, 34.6 so).
-        uint32_t h[4][16];
+        uint32_t h[kChunks][16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = half * 32 + 64 * i;
+        for (int i = 0; i < kChunks; ++i) {
+          const int c = half * 32 + kStride * i;
           if (c >= tl.ncols) break;
           uint32_t v[32];
           if (empty) {
@@ -719,7 +726,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           }
         }
         if (!empty) hand_back(acc);
-        // Through shared memory to 16-byte stores, two chunks at a time: a chunk as 32 rows (columns) of 64
+        // Through shared memory to 16-byte stores, kAtOnce chunks at a time: a chunk as 32 rows (columns) of 64
         // bytes, 16-byte pieces xor-swizzled by row pair.  Neighbouring lanes exchange halves first, so that
         // a lane stores the values of two features of one column (even lanes the even column): 128 bytes a
         // store without a bank conflict.  The MMA's operands come through the same shared memory.  (Two-byte
@@ -729,51 +736,51 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const int piece = lane & 3;
         const int mp = m - lane + piece * 8;  // (the extent is a multiple of 8: all of a piece or none)
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const int c = half * 32 + 64 * i;
+        for (int i = 0; i < kChunks; i += kAtOnce) {
+          const int c = half * 32 + kStride * i;
           if (c >= tl.ncols) break;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b == 1 && c + 64 >= tl.ncols) break;
+          for (int b = 0; b < kAtOnce; ++b) {
+            if (b == 1 && c + kStride >= tl.ncols) break;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const uint32_t other = __shfl_xor_sync(0xffffffffu, h[i + b][j], 1);
-              const uint32_t a = pair_base + b * (kGroupStage / 2) + j * 128 + (((lane >> 3) ^ (j & 3)) << 4);
+              const uint32_t a = pair_base + b * 2048 + j * 128 + (((lane >> 3) ^ (j & 3)) << 4);
               asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(__byte_perm(h[i + b][j], other, pick)) : "memory");
             }
           }
           __syncwarp();
           if (p.wide_rows) {
-            uint4 d[8];
+            uint4 d[4 * kAtOnce];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
+            for (int u = 0; u < 4 * kAtOnce; ++u) {
               const int row = (u & 3) * 8 + (lane >> 2);
               asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                            : "=r"(d[u].x), "=r"(d[u].y), "=r"(d[u].z), "=r"(d[u].w)
-                           : "r"(stage_base + (u >> 2) * (kGroupStage / 2) + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                           : "r"(stage_base + (u >> 2) * 2048 + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
                            : "memory");
             }
             if (mp < p.M) {
               uint16_t* out = static_cast<uint16_t*>(p.out) + first - lane + piece * 8 + (c + (lane >> 2)) * ldc;
               const int left = tl.ncols - c - (lane >> 2);
 #pragma unroll
-              for (int u = 0; u < 8; ++u) {
-                const int row = (u >> 2) * 64 + (u & 3) * 8;
+              for (int u = 0; u < 4 * kAtOnce; ++u) {
+                const int row = (u >> 2) * kStride + (u & 3) * 8;
                 if (row < left) *reinterpret_cast<uint4*>(out + row * ldc) = d[u];
               }
             }
           } else {
             // rows of any length and alignment: a value a lane.  (Rolled: 32 stores a chunk written out, straight
             // from the registers, cost 1003 rows of 1001 features 4250 cycles a tile, mostly instruction fetch.)
-            for (int b = 0; b < 2; ++b) {
-              const int rows = min(tl.ncols - c - 64 * b, 32);
-              uint16_t* out = static_cast<uint16_t*>(p.out) + first + (c + 64 * b) * ldc;
+            for (int b = 0; b < kAtOnce; ++b) {
+              const int rows = min(tl.ncols - c - kStride * b, 32);
+              uint16_t* out = static_cast<uint16_t*>(p.out) + first + (c + kStride * b) * ldc;
 #pragma unroll 4
               for (int row = 0; row < rows; ++row, out += ldc) {
                 uint16_t d;
                 asm volatile("ld.shared.u16 %0, [%1];"
                              : "=h"(d)
-                             : "r"(stage_base + b * (kGroupStage / 2) + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) << 4) + (lane & 7) * 2)
+                             : "r"(stage_base + b * 2048 + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) << 4) + (lane & 7) * 2)
                              : "memory");
                 if (mine) *out = d;
               }

@@ -58,7 +58,10 @@ bool setup_device(Driver* d) {
   if (prop.major != 10) return false;
   d->sm_count = prop.multiProcessorCount;
   // Opt in to the large dynamic shared-memory carve-out for every kernel instantiation.
-  const void* kernels[40] = {
+  const void* kernels[43] = {
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1, false, true>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kDx, 1, false, true>),
+      reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 1, false, true>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 2>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kFwd, 1, true>),
       reinterpret_cast<const void*>(&hb::hb_group_kernel<hb::kMx, 1, true>),
@@ -101,6 +104,11 @@ bool setup_device(Driver* d) {
       reinterpret_cast<const void*>(&hb::hb_conv_strip_kernel<2, 0, 1>)};
   for (const void* k : kernels)
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit) != cudaSuccess)
+      return false;
+  // (the first three: two CTAs to an SM need all of its shared memory)
+  for (int i = 0; i < 3; ++i)
+    if (cudaFuncSetAttribute(kernels[i], cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return false;
   return true;
 }
@@ -395,7 +403,7 @@ struct hb_plan {
   // products grouped by expert and 4-bit products: tmA, and the token matrix in boxes of 64 rows (tmB), of 16
   // (tmB2) and of a whole tile (tmC);
   // group_zero_bytes: no rows at all, the weight gradient is cleared and nothing is launched
-  bool group;
+  bool group, group_narrow;
   int group_mode;
   hb::GroupParams gp;
   size_t group_zero_bytes;

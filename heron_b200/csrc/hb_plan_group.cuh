@@ -15,8 +15,9 @@ struct GroupProblem {
 };
 
 // (split: the buffer in which the CTAs of a cluster join their sums, 128 lanes x 64 columns)
-int group_fixed_smem(int E, bool split = false) {
-  return (split ? hb::kTileM * 64 * 4 : 0) + 1024 /*alignment of the ring*/ + hb::kGroupEpi * hb::kGroupStage + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
+int group_fixed_smem(int E, bool split = false, bool narrow = false) {
+  return (split ? hb::kTileM * 64 * 4 : 0) + 1024 /*alignment of the ring*/ +
+         hb::group_epi(narrow) * hb::group_staging(narrow) + static_cast<int>((sizeof(hb::GroupBars) + 15) & ~15) +
          E * static_cast<int>(sizeof(hb::GroupEntry));
 }
 
@@ -39,7 +40,25 @@ int group_tmem(const GroupProblem& g, const hb_knobs& k) {
   return c;
 }
 
-void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
+// The narrow form, two CTAs to an SM (tiles of 64 columns, four epilogue warps, rings half as deep): one's
+// set-up, epilogue and issuing pass under the other's loads, and twice as many tiles find a place at once.
+// Measured, wide / narrow: MXFP4 16 rows over 32 experts of 2048 x 2048 10.8 / 8.5 us, 256 rows 19.0 / 16.1, 1024 rows over
+// 128 of 1024 x 2048 31.7 / 29.1; fp16 1003 rows over 24 experts of 1001 x 712 13.0 / 12.1, bf16 256 rows over 32 of
+// 2048 x 2048 45.0 / 43.7.  16-bit operands lose where all tiles find an SM of their own (256 rows over 8 experts 15.2 / 16.5,
+// unless the reduction is short: dx with 328 features 6.1 / 5.8) and where there are many rounds (1024 rows over 128
+// experts 82.4 / 83.8): the deeper ring is worth more there.
+constexpr int kNarrowSmem = (233472 - 2 * 1024) / 2;  // an SM's shared memory less what the system keeps of a CTA's
+bool is_narrow(const GroupProblem& g, const hb_knobs& k, int sms) {
+  if (g.mode == hb::kDw || k.tile_n != 64 || k.cta_group != 1 || k.split_k != 1 || k.max_ctas != 0) return false;
+  const int elems = g.mode == hb::kMx ? 256 : 64;
+  // (tiles to expect: a row in every group, or as many groups as rows)
+  const long long tiles = static_cast<long long>(g.T < g.E ? g.T : g.E) * ((g.M + hb::kTileM - 1) / hb::kTileM);
+  if (tiles <= sms && (g.R + elems - 1) / elems > 8) return false;
+  if (g.mode != hb::kMx && tiles > 6LL * sms) return false;
+  return group_fixed_smem(g.E, false, true) + (k.stages > 0 ? k.stages : 2) * group_stage(g, 64, 1) <= kNarrowSmem;
+}
+
+void group_knobs(const GroupProblem& g, const hb_knobs* in, int sms, hb_knobs* out) {
   hb_knobs k;
   if (in) k = *in; else std::memset(&k, 0, sizeof(k));
   const int avg = g.T / g.E;  // mean rows of a group
@@ -70,12 +89,13 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, hb_knobs* out) {
     k.split_k = 1;
     if ((g.mode == hb::kFwd || g.mode == hb::kMx) && k.cta_group == 1 && k.tile_n == 64) {
       const int elems = g.mode == hb::kMx ? 256 : 64;
-      const int sms = k.max_ctas > 0 && k.max_ctas < 148 ? k.max_ctas : 148;
+      const int most = k.max_ctas > 0 && k.max_ctas < sms ? k.max_ctas : sms;
       if ((g.R + elems - 1) / elems >= 32)
-        while (k.split_k < 4 && most_tiles(g, k) * k.split_k * 2 <= sms) k.split_k *= 2;
+        while (k.split_k < 4 && most_tiles(g, k) * k.split_k * 2 <= most) k.split_k *= 2;
     }
   }
-  const int room = kSmemLimit - group_fixed_smem(g.E, k.split_k > 1);
+  const bool narrow = is_narrow(g, k, sms);
+  const int room = (narrow ? kNarrowSmem : kSmemLimit) - group_fixed_smem(g.E, k.split_k > 1, narrow);
   if (k.stages == 0) {
     k.stages = room / group_stage(g, k.tile_n, k.cta_group);
     // (kMx: TMEM columns of the scales beside two accumulators, or one where two leave none)
@@ -162,7 +182,7 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   Driver& d = driver();
   if (d.status != HB_OK) return d.status;
   hb_knobs k;
-  group_knobs(g, knobs, &k);
+  group_knobs(g, knobs, d.sm_count, &k);
   int rc = check_group_knobs(g, k);
   if (rc != HB_OK) return rc;
   if ((!knobs || !knob_names_tiles(*knobs)) && few_rows(g)) {
@@ -208,13 +228,15 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   }
   const long long tiles = most_tiles(g, k);
   if (tiles > 0x3fffffffLL) return HB_ERR_SHAPE;
+  const bool narrow = is_narrow(g, k, d.sm_count);
+  plan->group_narrow = narrow;
   const int together = k.cta_group * k.split_k;  // CTAs of a cluster
-  int units = d.sm_count / together;
+  int units = d.sm_count * (narrow ? 2 : 1) / together;
   if (k.max_ctas > 0 && k.max_ctas / together < units) units = k.max_ctas / together;
   if (units < 1) units = 1;
   plan->grid = static_cast<int>(tiles < units ? tiles : units) * together;
   p.ksplit = k.split_k;
-  plan->smem = group_fixed_smem(g.E, k.split_k > 1) + k.stages * group_stage(g, k.tile_n, k.cta_group);
+  plan->smem = group_fixed_smem(g.E, k.split_k > 1, narrow) + k.stages * group_stage(g, k.tile_n, k.cta_group);
   plan->knobs = k;
 
   const uint64_t T = g.T, E = g.E, M = g.M, R = g.R, C = g.C;
@@ -270,12 +292,12 @@ int plan_mx(const void* x, const void* x_scales, const void* w, const void* w_sc
   return plan_group(g, w, x, out, w_scales, x_scales, offsets, knobs, plan);
 }
 
-template <int MODE, int CG, bool SPLIT = false>
+template <int MODE, int CG, bool SPLIT = false, bool NARROW = false>
 int launch_group(const hb_plan* plan, cudaStream_t stream) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(plan->grid);
-  cfg.blockDim = dim3(hb::group_threads(MODE));
+  cfg.blockDim = dim3(hb::group_threads(MODE, NARROW));
   cfg.dynamicSmemBytes = plan->smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -285,7 +307,7 @@ int launch_group(const hb_plan* plan, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG, SPLIT>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->tmSA, plan->tmSB, plan->gp);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, hb::hb_group_kernel<MODE, CG, SPLIT, NARROW>, plan->tmA, plan->tmB, plan->tmB2, plan->tmC, plan->tmSA, plan->tmSB, plan->gp);
   return e == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
@@ -318,6 +340,13 @@ int run_group(const hb_plan* plan, cudaStream_t stream) {
   if (plan->gp.ksplit > 1)
     return plan->group_mode == hb::kFwd ? launch_group<hb::kFwd, 1, true>(plan, stream)
                                         : launch_group<hb::kMx, 1, true>(plan, stream);
+  if (plan->group_narrow) {
+    switch (plan->group_mode) {
+      case hb::kFwd: return launch_group<hb::kFwd, 1, false, true>(plan, stream);
+      case hb::kDx: return launch_group<hb::kDx, 1, false, true>(plan, stream);
+      default: return launch_group<hb::kMx, 1, false, true>(plan, stream);
+    }
+  }
   switch (plan->group_mode) {
     case hb::kFwd: return pair ? launch_group<hb::kFwd, 2>(plan, stream) : launch_group<hb::kFwd, 1>(plan, stream);
     case hb::kDx: return pair ? launch_group<hb::kDx, 2>(plan, stream) : launch_group<hb::kDx, 1>(plan, stream);
