@@ -126,18 +126,23 @@ int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
   return HB_OK;
 }
 
-// Whether a product is left to the kernels that stream the weights (hb_rows.cuh).  Measured against the tile
-// kernel: bf16, 1 and 8 rows x 4096 x 4096 7.0 and 8.4 / 17.0 us (with its reduction over a cluster 10.4), 16
-// rows (two passes) 16.9 / 11; 16 and 32 rows over 32 experts of 2048 x 2048 20.8 and 30.8 / 22.6 and 32.9, 16 rows
-// over 8 13.9 / 13.1.  MXFP4, whose kernel is bound by widening elements, by the weights of all passes: 16.8
-// million 6.9 / 9.3 us (one row, 4096 x 4096) and 7.0 / 7.1 (four rows to four experts of 2048 x 2048), twice as
-// many 10.2 / 7.4; and a long reduction over few features is one for the cluster (1024 x 16384 13 / 8.4).
+// Whether a product is left to the kernels that stream the weights (hb_rows.cuh), by the weights that all their
+// passes read: one pass for eight rows of a group, so one for up to eight rows of a single group, and at worst
+// one for every row where there are more groups.  Measured, streaming / tiles (with a cluster or two CTAs to an
+// SM where those are chosen):
+//   bf16, one group: 16.8 million weights in one pass (8 rows, 4096 x 4096) 8.3 / 10.9 us, 67 million (one row) 25.6 /
+//   26.6; two passes of 16.8 million 15.0 / 11.2, three of 2.1 million (24 rows) 5.3 / 7.6
+//   bf16, rows over 32 experts of 2048 x 2048: 4 rows 6.6 / 9.4, 8 rows 14.5 / 13.7, 16 rows 20.8 / 21.0, 24 rows 27.2 /
+//   27.9 (the memory's time either way); 16 rows over 8 experts 13.9 / 13.0
+//   MXFP4, bound by widening elements: one group, 16.8 million in one pass 6.9 - 8.3 / 8.4, two of 2.1 million 5.2 / 5.8
+//   or (256 x 8192) 11.5 / 8.3; 8.4 million in two or four rows to experts of their own 4.7 and 5.2 / 5.8 and 6.6, 16.8 million 7.7 / 6.4
+// (at most 64 rows: all of them in one group are then eight passes over its weights)
 bool few_rows(const GroupProblem& g) {
-  // (at most 64 rows: all of them in one group are then eight passes over its weights)
-  if (g.mode == hb::kFwd) return g.T <= (g.E > 64 ? 64 : (g.E > 8 ? g.E : 8));
-  if (g.mode != hb::kMx || g.T > 64 || g.R > 8192) return false;
-  const long long passes = g.E == 1 ? (g.T + 7) / 8 : g.T;
-  return passes * g.M * g.R <= (1LL << 24);
+  if ((g.mode != hb::kFwd && g.mode != hb::kMx) || g.T > 64) return false;
+  const long long weights = static_cast<long long>(g.M) * g.R;
+  if (g.mode == hb::kMx) return g.R <= 8192 && (g.E == 1 ? g.T <= 8 && weights <= (1LL << 24) : g.T * weights <= (1LL << 23));
+  if (g.E == 1) return g.T <= 8 || (g.T + 7) / 8 * weights <= (1LL << 23);
+  return g.T <= (g.E > 8 ? g.E : 8);
 }
 
 // Knobs of the tile kernel, given by the caller: then that kernel is meant.
