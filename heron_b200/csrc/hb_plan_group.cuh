@@ -131,7 +131,8 @@ int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
 // one for every row where there are more groups.  Measured, streaming / tiles (with a cluster or two CTAs to an
 // SM where those are chosen):
 //   bf16, one group: 16.8 million weights in one pass (8 rows, 4096 x 4096) 8.3 / 10.9 us, 67 million (one row) 25.6 /
-//   26.6; two passes of 16.8 million 15.0 / 11.2, three of 2.1 million (24 rows) 5.3 / 7.6
+//   26.6, but of 8192 and more features, whose tiles fill the SMs, 8 rows 19.2 / 16.7 (K 4096) and one row x 14336 x 4096
+//   27.2 / 21.7; two passes of 16.8 million 15.0 / 11.2, three of 2.1 million (24 rows) 5.3 / 7.6
 //   bf16, rows over 32 experts of 2048 x 2048: 4 rows 6.6 / 9.4, 8 rows 14.5 / 13.7, 16 rows 20.8 / 21.0, 24 rows 27.2 /
 //   27.9 (the memory's time either way); 16 rows over 8 experts 13.9 / 13.0
 //   MXFP4, bound by widening elements: one group, 16.8 million in one pass 6.9 - 8.3 / 8.4, two of 2.1 million 5.2 / 5.8
@@ -141,7 +142,7 @@ bool few_rows(const GroupProblem& g) {
   if ((g.mode != hb::kFwd && g.mode != hb::kMx) || g.T > 64) return false;
   const long long weights = static_cast<long long>(g.M) * g.R;
   if (g.mode == hb::kMx) return g.R <= 8192 && (g.E == 1 ? g.T <= 8 && weights <= (1LL << 24) : g.T * weights <= (1LL << 23));
-  if (g.E == 1) return g.T <= 8 || (g.T + 7) / 8 * weights <= (1LL << 23);
+  if (g.E == 1) return (g.T <= 8 && g.M <= 4096) || (g.T + 7) / 8 * weights <= (1LL << 23);
   return g.T <= (g.E > 8 ? g.E : 8);
 }
 
