@@ -112,6 +112,13 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, int sms, hb_knobs* o
   *out = k;
 }
 
+// What the caller gave, before defaults are worked out from it (sizes of a ring stage are divided by).
+bool group_knobs_in_range(const hb_knobs& k) {
+  return k.tile_n >= 0 && k.tile_n <= 256 && k.tile_n % 64 == 0 && k.cta_group >= 0 && k.cta_group <= 2 && k.split_k >= 0 &&
+         k.split_k <= 8 && k.stages >= 0 && k.stages <= hb::kMaxStages && k.acc_stages >= 0 && k.acc_stages <= 2 &&
+         k.max_ctas >= 0;
+}
+
 int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
   if (k.cta_group != 1 && k.cta_group != 2) return HB_ERR_KNOB;
   if (k.cta_group == 2 && g.mode == hb::kDw) return HB_ERR_KNOB;
@@ -185,6 +192,7 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   if (mx && (!sfa || !sfb || !aligned16(sfa) || !aligned16(sfb))) return HB_ERR_ALIGN;
   if (!offsets && !(mx && g.E == 1)) return HB_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) return HB_ERR_ALIGN;
+  if (knobs && !group_knobs_in_range(*knobs)) return HB_ERR_KNOB;
   Driver& d = driver();
   if (d.status != HB_OK) return d.status;
   hb_knobs k;

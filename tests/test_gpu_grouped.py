@@ -243,6 +243,20 @@ def test_gradients_against_differences(K):
     assert abs(((up - down) * dy.double()).sum() - 2 * (dw.double() * vw.double()).sum()) <= tol
 
 
+def test_plans_report_their_knobs(K):
+    x, w, dy, _, offsets = make(6, [40, 3, 90], 0, 0, 128, 192, torch.bfloat16)
+    for plan in (K.plan_grouped_gemm(x, w, offsets), K.plan_grouped_gemm_dx(dy, w, offsets),
+                 K.plan_grouped_gemm_dw(dy, x, offsets)):
+        k = plan.knobs()
+        assert k["tile_n"] in (64, 128, 192, 256) and k["stages"] >= 1 and k["grid"] >= 1 and k["smem_bytes"] <= 232448
+    few = K.plan_grouped_gemm(x[:3].contiguous(), w, offsets)
+    assert few.knobs()["tile_n"] == 0  # a kernel without tiles
+    for bad in (dict(tile_n=64, split_k=3), dict(tile_n=128, split_k=2), dict(tile_n=64, cta_group=2), dict(tile_n=256, stages=12)):
+        from heron_b200._lib import HeronB200Error
+        with pytest.raises(HeronB200Error):
+            K.plan_grouped_gemm(x, w, offsets, knobs=bad)
+
+
 def test_a_silent_producer_ends_in_a_status(K):
     """The bounded waits: nothing is loaded, the launch ends by itself and reports it."""
     from heron_b200 import _lib

@@ -36,6 +36,18 @@ def test_grouped_argument_errors(hb_lib, ptrs):
     assert hb_lib.hb_grouped_gemm_dw(None, None, None, p, 0, 64, 64, 2, F16, F32, None, None) == _lib.HB_ERR_ALIGN
 
 
+@pytest.mark.parametrize("bad", [dict(tile_n=-128), dict(tile_n=(1 << 25) - 128), dict(tile_n=96), dict(tile_n=320),
+                                 dict(cta_group=3), dict(cta_group=-1), dict(split_k=-1), dict(split_k=9), dict(stages=-1),
+                                 dict(stages=13), dict(acc_stages=3), dict(max_ctas=-1)])
+def test_knobs_out_of_range(hb_lib, ptrs, bad):
+    from heron_b200 import _lib
+    _, p, _, _ = ptrs
+    k = ctypes.byref(_lib.HbKnobs.from_dict(bad))
+    for fn in (hb_lib.hb_grouped_gemm, hb_lib.hb_grouped_gemm_dx, hb_lib.hb_grouped_gemm_dw):
+        assert fn(p, p, p, p, 16, 64, 64, 2, _lib.HB_F16, _lib.HB_F32, k, None) == _lib.HB_ERR_KNOB
+    assert hb_lib.hb_gemm_mxfp4(p, p, p, p, p, 4, 64, 8, _lib.HB_F32, k, None) == _lib.HB_ERR_KNOB
+
+
 def test_the_other_operators_keep_refusing_bfloat16(hb_lib, ptrs):
     from heron_b200 import _lib
     _, p, _, _ = ptrs
