@@ -280,10 +280,16 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   return rc;
 }
 
+// The kernels round sizes up to whole tiles in 32 bits.
+constexpr int kMostSize = 1 << 30;
+bool sizes_ok(int T, int K, int N, int E) {
+  return T >= 0 && T <= kMostSize && K > 0 && K <= kMostSize && N > 0 && N <= kMostSize && E > 0 && E <= hb::kMaxGroups;
+}
+
 int plan_grouped(int mode, const void* A, const void* B, void* out, const int* offsets, int T, int K, int N, int E,
                  hb_dtype in, hb_dtype out_t, const hb_knobs* knobs, hb_plan* plan) {
   std::memset(plan, 0, sizeof(*plan));
-  if (T < 0 || K <= 0 || N <= 0 || E <= 0 || E > hb::kMaxGroups) return HB_ERR_SHAPE;
+  if (!sizes_ok(T, K, N, E)) return HB_ERR_SHAPE;
   if ((in != HB_F16 && in != HB_BF16) || out_type_of(out_t) < 0) return HB_ERR_DTYPE;
   // row pitches of the operands are multiples of 16 bytes (the output's need not be)
   if (K % 8 != 0 || (mode != hb::kFwd && N % 8 != 0)) return HB_ERR_SHAPE;
@@ -298,7 +304,7 @@ int plan_grouped(int mode, const void* A, const void* B, void* out, const int* o
 int plan_mx(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, const int* offsets,
             int T, int K, int N, int E, hb_dtype out_t, const hb_knobs* knobs, hb_plan* plan) {
   std::memset(plan, 0, sizeof(*plan));
-  if (T < 0 || K <= 0 || N <= 0 || E <= 0 || E > hb::kMaxGroups || K % 32 != 0) return HB_ERR_SHAPE;
+  if (!sizes_ok(T, K, N, E) || K % 32 != 0) return HB_ERR_SHAPE;
   if (out_type_of(out_t) < 0) return HB_ERR_DTYPE;
   GroupProblem g;
   g.mode = hb::kMx; g.T = T; g.E = E; g.in = HB_U8; g.out = out_t;

@@ -317,7 +317,8 @@ int hb_conv2d_nhwc_packed_noalloc(const void* in, const void* w_packed, void* ou
  *                                                                         without rows
  * in: HB_F16 or HB_BF16 for both operands; out: HB_F32, HB_F16 or HB_BF16.  fp32 accumulation in a
  * fixed order, one rounding at the end.  Dense row-major buffers; K % 8 == 0, for the gradients
- * also N % 8 == 0; 1 <= E <= 1024; T >= 0 (T = 0: only the weight gradient is written).
+ * also N % 8 == 0; 1 <= E <= 1024; T >= 0 (T = 0: only the weight gradient is written); T, K and N up
+ * to 2^30.
  * Knobs used: tile_n (64, 128, 192, 256: the widest tile of a group's rows; of N in dw), stages,
  * acc_stages, cta_group (2: not dw, tile_n at least 128), split_k (1, 2, 4, 8: CTAs of a cluster that share
  * the reduction of a tile; forward products with tile_n 64 and cta_group 1), max_ctas, silent_producer; the

@@ -48,6 +48,19 @@ def test_knobs_out_of_range(hb_lib, ptrs, bad):
     assert hb_lib.hb_gemm_mxfp4(p, p, p, p, p, 4, 64, 8, _lib.HB_F32, k, None) == _lib.HB_ERR_KNOB
 
 
+@pytest.mark.parametrize("n", [2 ** 30 + 32, 2 ** 31 - 32])
+def test_sizes_whose_round_up_would_wrap(hb_lib, ptrs, n):
+    """Sizes are rounded up to whole tiles in 32 bits: what could wrap is refused."""
+    from heron_b200 import _lib
+    _, p, _, _ = ptrs
+    F16, F32 = _lib.HB_F16, _lib.HB_F32
+    for T, K, N in ((n, 64, 64), (16, n, 64), (16, 64, n)):
+        for fn in (hb_lib.hb_grouped_gemm, hb_lib.hb_grouped_gemm_dx, hb_lib.hb_grouped_gemm_dw):
+            assert fn(p, p, p, p, T, K, N, 2, F16, F32, None, None) == _lib.HB_ERR_SHAPE
+        assert hb_lib.hb_gemm_mxfp4(p, p, p, p, p, T, K, N, F32, None, None) == _lib.HB_ERR_SHAPE
+        assert hb_lib.hb_grouped_gemm_mxfp4(p, p, p, p, p, p, T, K, N, 2, F32, None, None) == _lib.HB_ERR_SHAPE
+
+
 def test_the_other_operators_keep_refusing_bfloat16(hb_lib, ptrs):
     from heron_b200 import _lib
     _, p, _, _ = ptrs
