@@ -185,18 +185,26 @@ __device__ __forceinline__ void widen_e2m1x8(uint32_t w, uint32_t (&h)[4]) {
   h[3] = (w & 0x80008000u) | ((w >> 3) & 0x0e000e00u);
 }
 
-// The values of a scale word's four bytes (E8M0).  0 (2^-127, subnormal) and 255 (NaN) are rare and take
-// three more operations a byte.
+// Whether one of four scale bytes (E8M0) is 160 or more: 2^33 on, and NaN.
+__device__ __forceinline__ bool e8m0_far(uint32_t word) { return (word & ((word << 1) | (word << 2)) & 0x80808080u) != 0u; }
+
+// The values of four scale bytes that are not far, times 2^14 (so that byte 0, 2^-127, is a normal number too).
 __device__ __forceinline__ void e8m0_values(uint32_t word, float (&v)[4]) {
-  uint32_t b[4] = {(word << 23) & 0x7f800000u, (word << 15) & 0x7f800000u, (word << 7) & 0x7f800000u,
-                   (word >> 1) & 0x7f800000u};
-  if ((((word - 0x01010101u) & ~word) | ((~word - 0x01010101u) & word)) & 0x80808080u) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (b[i] == 0u || b[i] == 0x7f800000u) b[i] |= 0x00400000u;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(b[i]);
+  constexpr uint32_t k14 = 14u << 23;
+  v[0] = __uint_as_float(((word << 23) & 0x7f800000u) + k14);
+  v[1] = __uint_as_float(((word << 15) & 0x7f800000u) + k14);
+  v[2] = __uint_as_float(((word << 7) & 0x7f800000u) + k14);
+  v[3] = __uint_as_float(((word >> 1) & 0x7f800000u) + k14);
+}
+
+// sum + d 2^28 2^(a - 127) 2^(b - 127) for any two scale bytes, 255 being NaN.  d 2^28 is a multiple of 1/4 with 13 bits;
+// the exponents are added as integers and half of their sum is applied at a time (2^-127 is subnormal), so that nothing
+// leaves fp32 on the way unless the result does, and the only rounding is that of the sum.
+__device__ __forceinline__ float add_far(float d, uint32_t a, uint32_t b, float sum) {
+  const int e = static_cast<int>(a + b) - 254, h = e >> 1;
+  auto power = [](int n) { return __uint_as_float(n > -127 ? static_cast<uint32_t>(n + 127) << 23 : 0x00400000u); };
+  const float s = a == 255u || b == 255u ? __uint_as_float(0x7fc00000u) : power(e - h);
+  return fmaf(d * 268435456.f * power(h), s, sum);
 }
 
 // d (16 x 8, fp32) = a (16 x 16, fp16) * b (16 x 8, fp16)
@@ -211,10 +219,13 @@ __device__ __forceinline__ void mma_16x8x16_from_zero(float (&d)[4], uint32_t a0
 // MXFP4 operands.  A lane's 16 bytes are one block of 32 elements; four lanes exchange them so that each
 // holds a quarter of every block, and a block is two instructions in fp16 from zero: the elements' products
 // are multiples of 1/4 up to 36 (times 2^-28), so the block's sum has 13 bits and is exact.  It is
-// multiplied by the product of the two scales and added in fp32; 2^28 is put back at the end.  The
-// instructions bound the kernel (400 for 16 x 128 weights, 0.53 issued a cycle and scheduler), not the
-// memory; the conversion instruction for two elements and E4M3 operands for the 32-deep instruction were
-// no faster than the bit operations here.  A warp takes tiles of 128 elements, kRowsWarps tiles apart.
+// multiplied by the product of the two scales, each times 2^14, and added in fp32.  That product is below 2^93 as long
+// as no scale passes 2^32, and it is exact down to 2^-149, below which a block's true sum is under 2^-166 and lost in any
+// fp32 sum.  A warp that meets a larger scale takes the longer way of add_far for the tile: scales of 2^64 would meet
+// in an infinity where the sum is 2^126 or 0.  (2^28 put back at the end kept sums below 2^-98 in subnormals.)
+// The instructions bound the kernel (about 400 for 16 x 128 weights), not the memory: one row of 4096 x 4096
+// 7.0 us, eight 7.6 (with the choice made inside the loop over blocks 7.4 and 7.9); the conversion
+// instruction for two elements and E4M3 operands for the 32-deep instruction were no faster than the bit operations here.  A warp takes tiles of 128 elements, kRowsWarps tiles apart.
 // The 16 features are four lines of the scale tile in each of its four bands: their scales of 128 elements
 // are 64 consecutive bytes (16 features in a row would use a quarter of every sector).
 __global__ void __launch_bounds__(kRowsWarps * 32) hb_mx_rows_kernel(const RowsParams p) {
@@ -253,8 +264,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32) hb_mx_rows_kernel(const RowsP
       const bool in = i < kt;
       sa[u] = in ? wsf[i * (kAtomBytes / 4)] : 0u;
       sb[u] = in ? wsf[i * (kAtomBytes / 4) + 8] : 0u;  // (feature g + 8: two lines on)
-      s0[u] = in && 2 * c < rows ? xsf[i * (kAtomBytes / 4) + 8 * c] : 0u;
-      s1[u] = in && 2 * c + 1 < rows ? xsf[i * (kAtomBytes / 4) + 8 * c + 4] : 0u;
+      // (columns without a row: scales of 1, which are not far)
+      s0[u] = in && 2 * c < rows ? xsf[i * (kAtomBytes / 4) + 8 * c] : 0x7f7f7f7fu;
+      s1[u] = in && 2 * c + 1 < rows ? xsf[i * (kAtomBytes / 4) + 8 * c + 4] : 0x7f7f7f7fu;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -264,29 +276,46 @@ __global__ void __launch_bounds__(kRowsWarps * 32) hb_mx_rows_kernel(const RowsP
       transpose4(t[u], c);
       const uint32_t wa[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, wb[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
       const uint32_t wt[4] = {t[u].x, t[u].y, t[u].z, t[u].w};
-      float fa[4], fb[4], f0[4], f1[4];
-      e8m0_values(sa[u], fa);
-      e8m0_values(sb[u], fb);
-      e8m0_values(s0[u], f0);
-      e8m0_values(s1[u], f1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      const bool far = __any_sync(0xffffffffu, e8m0_far(sa[u]) || e8m0_far(sb[u]) || e8m0_far(s0[u]) || e8m0_far(s1[u]));
+      // block k of the tile: its sum over each pair of a feature and a token, times 2^-28
+      auto block_sums = [&](int k, float (&d)[4]) {
         uint32_t ha[4], hb[4], ht[4];
         widen_e2m1x8(wa[k], ha);
         widen_e2m1x8(wb[k], hb);
         widen_e2m1x8(wt[k], ht);
-        float d[4];
         mma_16x8x16_from_zero(d, ha[0], hb[0], ha[1], hb[1], ht[0], ht[1]);
         mma_16x8x16<1>(d, ha[2], hb[2], ha[3], hb[3], ht[2], ht[3]);
-        acc[0] = fmaf(d[0], fa[k] * f0[k], acc[0]);
-        acc[1] = fmaf(d[1], fa[k] * f1[k], acc[1]);
-        acc[2] = fmaf(d[2], fb[k] * f0[k], acc[2]);
-        acc[3] = fmaf(d[3], fb[k] * f1[k], acc[3]);
+      };
+      if (!far) {
+        float fa[4], fb[4], f0[4], f1[4];
+        e8m0_values(sa[u], fa);
+        e8m0_values(sb[u], fb);
+        e8m0_values(s0[u], f0);
+        e8m0_values(s1[u], f1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float d[4];
+          block_sums(k, d);
+          acc[0] = fmaf(d[0], fa[k] * f0[k], acc[0]);
+          acc[1] = fmaf(d[1], fa[k] * f1[k], acc[1]);
+          acc[2] = fmaf(d[2], fb[k] * f0[k], acc[2]);
+          acc[3] = fmaf(d[3], fb[k] * f1[k], acc[3]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float d[4];
+          block_sums(k, d);
+          const uint32_t a0 = (sa[u] >> (8 * k)) & 255u, b0 = (sb[u] >> (8 * k)) & 255u;
+          const uint32_t t0 = (s0[u] >> (8 * k)) & 255u, t1 = (s1[u] >> (8 * k)) & 255u;
+          acc[0] = add_far(d[0], a0, t0, acc[0]);
+          acc[1] = add_far(d[1], a0, t1, acc[1]);
+          acc[2] = add_far(d[2], b0, t0, acc[2]);
+          acc[3] = add_far(d[3], b0, t1, acc[3]);
+        }
       }
     }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] *= 268435456.f;
   rows_join<kRowsWarps>(p, acc, rows, r, feature);
 }
 

@@ -308,3 +308,61 @@ def test_expert_layer_in_training_and_serving(K):
         want, mag, _ = grouped(xv, wv, off)
         assert_product(y4, want, mag, k, "y4")
         assert torch.equal(xv.double().cpu(), quantise(x)[2])
+
+
+def check_product(K, a, b, what):
+    """gemm_mxfp4 of two matrices against 64 bits, in 32 and 16 bits out."""
+    a, b = K.quantize_mxfp4(a), K.quantize_mxfp4(b)
+    av, bv = K.dequantize_mxfp4(*a), K.dequantize_mxfp4(*b)
+    want, mag, _ = grouped(av, bv[None], [0, av.shape[0]])
+    for od in (torch.float32, torch.bfloat16):
+        assert_product(K.gemm_mxfp4(*a, *b, out_dtype=od), want, mag, av.shape[1], "%s %s" % (what, od))
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 40])
+@pytest.mark.parametrize("k", [96, 1024])
+@pytest.mark.parametrize("ea,eb", [(-60, -60), (60, 60), (-70, -48), (-48, -70), (100, -100), (-100, 100), (120, -124),
+                                   (-30, -31), (31, 32), (33, 40), (-126, 100)])
+def test_product_of_scales_far_from_one(K, M, k, ea, eb):
+    """Results from 2^-120 to 2^120, which all output types but fp16 hold: no scale may leave fp32 on the way."""
+    a, b = randn(M + k, M, k, scale=2.0 ** ea), randn(7, 40, k, scale=k ** -0.5) * 2.0 ** eb
+    check_product(K, a, b, "2^%d x 2^%d" % (ea, eb))
+
+
+@pytest.mark.parametrize("M", [1, 5, 8, 9])
+def test_product_of_blocks_of_mixed_scales(K, M):
+    """Every block of 32 with an exponent of its own, some blocks zero."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+
+    def operand(seed, rows, k):
+        e = torch.randint(-60, 55, (rows, k // 32, 1), generator=g, device="cuda").float()
+        z = (torch.rand(rows, k // 32, 1, generator=g, device="cuda") < 0.8).float()
+        return (randn(seed, rows, k // 32, 32) * torch.exp2(e) * z).reshape(rows, k)
+    for k in (32, 160, 1056):
+        check_product(K, operand(1, M, k), operand(2, 50, k), "k %d" % k)
+
+
+@pytest.mark.parametrize("M", [1, 8, 9])
+def test_large_scales_and_small_sums(K, M):
+    """Blocks whose scales' product passes 2^128 while the sum of their elements' products is 0 or 1/4."""
+    for e, meet, want in ((66, 0.0, 0.0), (110, 0.0, 0.0), (64, 0.5, 2.0 ** 126), (-66, 0.5, 2.0 ** -134)):
+        a, b = torch.zeros(M, 64, device="cuda"), torch.zeros(20, 64, device="cuda")
+        a[:, 1], b[:, 2] = 4.0, 4.0  # the scales are 2^e
+        a[:, 5], b[:, 5] = meet, meet
+        a[:, 40], b[:, 50] = 4.0, 4.0
+        out = K.gemm_mxfp4(*K.quantize_mxfp4(a * 2.0 ** e), *K.quantize_mxfp4(b * 2.0 ** e))
+        assert (out == want).all(), (e, meet, out[0, 0].item())
+
+
+@pytest.mark.parametrize("M", [1, 5, 8])
+def test_nan_scale_of_few_rows(K, M):
+    """As test_nan_scale_makes_its_row_nan, in the kernel of few rows."""
+    a, b = randn(1, M, 416), randn(2, 40, 416)
+    b[9, 1], b[30, 400] = torch.inf, torch.nan
+    if M > 1:
+        a[3, 170] = torch.nan
+    out = K.gemm_mxfp4(*K.quantize_mxfp4(a), *K.quantize_mxfp4(b))
+    nan = torch.zeros(M, 40, dtype=torch.bool, device="cuda")
+    nan[:, [9, 30]] = True
+    nan[3:4] = M > 1
+    assert torch.equal(torch.isnan(out), nan) and torch.isfinite(out[~nan]).all()
