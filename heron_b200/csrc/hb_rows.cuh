@@ -15,7 +15,7 @@
 // their place four rows took twice the time of one.)
 //
 //   block (x, y): 16 features, and row y; the block of a group's rows 8 i, of which it takes up to eight,
-//   works, the others leave at once.  The grid depends on T, not on E or the offsets.
+//   works, the others leave at once (see rows_taken).  The grid depends on T, not on E or the offsets.
 #pragma once
 #include "hb_mx.cuh"
 
@@ -37,14 +37,17 @@ struct RowsParams {
   long long w_matrix_sf;  // scale bytes of one expert
 };
 
-// The group that row r belongs to, by its clamped range (the first of several); false for none.  All
-// lanes take part and get the answer.
-__device__ __forceinline__ bool rows_group(const RowsParams& p, int r, int& e, int& start, int& end) {
+// The rows r .. r + rows - 1 that the block of row r takes, all of group e (by clamped ranges, the first group
+// that claims r); 0 for a block that leaves.  All lanes take part and get the answer.  A block works for a group's
+// rows 0, 8, ..., and for a group's row behind one that another group claims first, up to the group's next
+// multiple of eight: with offsets out of order, [0, 6, 2, 8], rows 6 and 7 are the third group's alone, whose row 2
+// goes to the first.  So every row that some group claims is taken.
+__device__ __forceinline__ int rows_taken(const RowsParams& p, int r, int& e, int& start) {
   e = 0;
   start = 0;
-  end = p.T;
-  if (!p.offsets) return true;
+  if (!p.offsets) return (r & (kRowsAtOnce - 1)) == 0 ? min(kRowsAtOnce, p.T - r) : 0;
   const int lane = threadIdx.x & 31;
+  bool other = false;  // row r - 1 is claimed by a group before this one
   for (int base = 0; base < p.E; base += 32) {
     const int g = base + lane;
     int s = 0, t = 0;
@@ -53,15 +56,19 @@ __device__ __forceinline__ bool rows_group(const RowsParams& p, int r, int& e, i
       t = min(max(p.offsets[g + 1], s), p.T);
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, s <= r && r < t);
+    const uint32_t above = __ballot_sync(0xffffffffu, s < r && r <= t);
     if (hit) {
       const int src = __ffs(hit) - 1;
       e = base + src;
       start = __shfl_sync(0xffffffffu, s, src);
-      end = __shfl_sync(0xffffffffu, t, src);
-      return true;
+      const int end = __shfl_sync(0xffffffffu, t, src);
+      const int into = (r - start) & (kRowsAtOnce - 1);
+      other |= (above & ((1u << src) - 1u)) != 0u;
+      return into == 0 || other ? min(kRowsAtOnce - into, end - r) : 0;
     }
+    other |= above != 0u;
   }
-  return false;
+  return 0;
 }
 
 // d (16 x 8, fp32) += a (16 x 16) * b (16 x 8).  TYPE: 1 fp16, 2 bf16
@@ -120,9 +127,9 @@ __global__ void __launch_bounds__(WARPS * 32) hb_group_rows_kernel(const RowsPar
   griddep_wait();
   griddep_launch_dependents();
   const int r = blockIdx.y;
-  int e, start, end;
-  if (!rows_group(p, r, e, start, end) || ((r - start) & (kRowsAtOnce - 1)) != 0) return;
-  const int rows = min(kRowsAtOnce, end - r);
+  int e, start;
+  const int rows = rows_taken(p, r, e, start);
+  if (rows == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int n0 = blockIdx.x * kRowsFeatures;
   // (rows behind the last feature read the last one and are not stored)
@@ -232,9 +239,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32) hb_mx_rows_kernel(const RowsP
   griddep_wait();
   griddep_launch_dependents();
   const int r = blockIdx.y;
-  int e, start, end;
-  if (!rows_group(p, r, e, start, end) || ((r - start) & (kRowsAtOnce - 1)) != 0) return;
-  const int rows = min(kRowsAtOnce, end - r);
+  int e, start;
+  const int rows = rows_taken(p, r, e, start);
+  if (rows == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int kt = (p.K + 127) / 128, blocks = p.K / 32;
   const int line0 = (blockIdx.x & 7) * 4, tile_n = blockIdx.x >> 3;
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) hb_mx_rows_kernel(const RowsP
   const uint32_t* wsf = reinterpret_cast<const uint32_t*>(p.w_sf + e * p.w_matrix_sf + static_cast<long long>(tile_n) * kt * kAtomBytes) +
                         (line0 + (g >> 2)) * 4 + (g & 3);
   const uint4* x = static_cast<const uint4*>(p.x) + static_cast<long long>(r + min(g, rows - 1)) * blocks;
-  // (a group's rows start at tile row start / 128 + e; eight rows from a multiple of eight share a band)
+  // (a group's rows start at tile row start / 128 + e; rows up to the next multiple of eight share a band)
   const int local = r - start;
   const uint32_t* xsf = reinterpret_cast<const uint32_t*>(
                             p.x_sf + static_cast<long long>((p.offsets ? start / 128 + e : 0) + local / 128) * kt * kAtomBytes) +

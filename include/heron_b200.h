@@ -347,6 +347,8 @@ int hb_grouped_gemm_dw(const void* dy, const void* x, void* dw, const int* offse
  * A batch of matrices (batch, rows, K) has one such scale array per matrix, one after the other.
  * With `groups` > 0 (and batch 1) the rows are grouped by `offsets` (device, groups + 1 ints, as in
  * hb_grouped_gemm) and group g's first tile row is offsets[g] / 128 + g; rows of no group are skipped.
+ * (Offsets out of order: the groups' tile rows have to rise with g and not to meet, or the rows concerned get
+ * arbitrary scales; nothing is read or written out of range.)
  * hb_mxfp4_scale_bytes gives the size of the scale array (0 for sizes the operators refuse).
  *
  * hb_quantize_mxfp4: in HB_F16, HB_BF16 or HB_F32.  hb_dequantize_mxfp4: the values, out HB_F32,

@@ -269,3 +269,29 @@ def test_a_silent_producer_ends_in_a_status(K):
         assert _lib.last_status() == _lib.HB_ERR_TIMEOUT
     want, mag, _ = grouped(x, w, off)
     assert_product(K.grouped_gemm(x, w, offsets), want, mag, 128)
+
+
+@pytest.mark.parametrize("knobs", [None, dict(tile_n=64), dict(tile_n=128, cta_group=2)])
+def test_overlapping_offsets(K, knobs):
+    """Offsets out of order whose ranges overlap: a row that one group owns is right, a row of two groups is one of the
+    two results, a row of none is untouched."""
+    from grouped_util import clamped
+    g = torch.Generator().manual_seed(3)
+    cases = [(8, [0, 6, 2, 8]), (8, [0, 5, 1, 8]), (8, [3, 7, 0, 6]), (20, [0, 11, 3, 20]), (40, [30, 9, 35, 2])]
+    cases += [(T, torch.randint(-2, T + 3, (E + 1,), generator=g).tolist()) for T, E in ((8, 5), (8, 8), (30, 41), (40, 64))]
+    for T, off in cases:
+        E = len(off) - 1
+        x, w, dy, _, _ = make(T + E, [T] + [0] * (E - 1), 0, 0, 264, 72, torch.bfloat16)
+        offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+        for fn, a, b in ((K.grouped_gemm, x, w), (K.grouped_gemm_dx, dy, w.transpose(1, 2))):
+            out = torch.full((T, b.shape[1]), 7.0, device="cuda")
+            fn(a, w, offsets, out=out, knobs=knobs)
+            near = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+            free = torch.ones(T, dtype=torch.bool, device="cuda")
+            for e, (s, t) in enumerate(clamped(off, T)):
+                want, mag, _ = grouped(a[s:t], b[e][None], [0, t - s])
+                k = a.shape[1]
+                near[s:t] |= (out[s:t].double() - want).abs() <= k * 2.0 ** -23 * mag
+                free[s:t] = False
+            assert near[~free].all(), "%s %s: rows %s" % (fn.__name__, off, (~near.all(1) & ~free).nonzero().flatten().tolist())
+            assert (out[free] == 7.0).all()

@@ -366,3 +366,27 @@ def test_nan_scale_of_few_rows(K, M):
     nan[:, [9, 30]] = True
     nan[3:4] = M > 1
     assert torch.equal(torch.isnan(out), nan) and torch.isfinite(out[~nan]).all()
+
+
+@pytest.mark.parametrize("k", [64, 416])
+def test_overlapping_offsets(K, k):
+    """Offsets out of order, groups' tiles of scales apart: rows that one group owns are right."""
+    from grouped_util import clamped
+    w = randn(7, 3, 40, k)
+    wc, ws = K.quantize_mxfp4(w)
+    wv = K.dequantize_mxfp4(wc, ws)
+    for off in ([0, 6, 2, 8], [0, 5, 1, 8], [3, 7, 0, 6], [2, 8, 3, 8]):
+        x = randn(6, 8, k)
+        offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+        xc, xs = K.quantize_mxfp4(x, offsets=offsets)
+        xv = quantise(x)[2].cuda()
+        for knobs in (None, dict(tile_n=64)):
+            out = torch.full((8, 40), 7.0, device="cuda")
+            K.grouped_gemm_mxfp4(xc, xs, wc, ws, offsets, out=out, knobs=knobs)
+            owners = torch.zeros(8, dtype=torch.int64)
+            for s, t in clamped(off, 8):
+                owners[s:t] += 1
+            once = (owners == 1).cuda()
+            want, mag, _ = grouped(xv, wv, off)
+            assert_product(out[once], want[once], mag[once], k, "%s %s" % (off, knobs))
+            assert (out[(owners == 0).cuda()] == 7.0).all()
