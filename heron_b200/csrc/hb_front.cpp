@@ -5,6 +5,9 @@
 // few microseconds, and the Python path costs 10.9 us a call (3.6 us of it for one fresh output, 2.4 us
 // for the checks, 1.2 us for ctypes; the launch itself 2.5 us).
 //
+// Python's lock is released while an output is allocated and the library called: both may wait (for memory, for room in
+// a stream's queue), and other threads, or a host function in that very queue, may need the lock meanwhile.
+//
 // Every function returns the result, an int (a status of the library that is not HB_OK), or None.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -48,22 +51,34 @@ int device_of(std::initializer_list<const at::Tensor*> ts) {
 
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 
-// The output: the caller's (if it is what the operator writes) or a fresh one; false: not for this path.
-bool output(PyObject* out, PyObject* dtype, at::IntArrayRef shape, const at::Tensor& like, at::Tensor* result) {
-  at::ScalarType want = at::kFloat;
+// For its lifetime other threads may run Python.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
+void allocate(at::Tensor* t, at::IntArrayRef shape, const at::Tensor& like, at::ScalarType type) {
+  if (!t->defined()) *t = at::empty(shape, like.options().dtype(type).requires_grad(false));
+}
+
+// The output: the caller's (if it is what the operator writes), or none yet and the type of a fresh one; false: not for
+// this path.
+bool output(PyObject* out, PyObject* dtype, at::IntArrayRef shape, int dev, at::Tensor* result, at::ScalarType* type) {
+  *type = at::kFloat;
   if (dtype != Py_None) {
     if (!THPDtype_Check(dtype)) return false;
-    want = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+    *type = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
   }
   if (out != Py_None) {
     const at::Tensor* t = dense(out);
-    if (!t || t->sizes() != shape || (dtype != Py_None && t->scalar_type() != want)) return false;
+    if (!t || t->sizes() != shape || t->get_device() != dev || (dtype != Py_None && t->scalar_type() != *type)) return false;
     *result = *t;
-    return code_of(t->scalar_type()) >= 0;
+    *type = t->scalar_type();
   }
-  if (code_of(want) < 0) return false;
-  *result = at::empty(shape, like.options().dtype(want).requires_grad(false));
-  return true;
+  return code_of(*type) >= 0;
 }
 
 PyObject* answer(int status, PyObject* out, const at::Tensor& result) {
@@ -101,12 +116,19 @@ PyObject* grouped(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int dev = device_of({x, w, off});
   if (dev < 0) Py_RETURN_NONE;
   at::Tensor out;
-  const int64_t shape[3] = {mode == 2 ? E : T, mode == 1 ? K : N, K};
-  if (!output(a[4], a[5], at::IntArrayRef(shape, mode == 2 ? 3 : 2), *x, &out) || out.get_device() != dev) Py_RETURN_NONE;
+  at::ScalarType type;
+  const int64_t sizes[3] = {mode == 2 ? E : T, mode == 1 ? K : N, K};
+  const at::IntArrayRef shape(sizes, mode == 2 ? 3 : 2);
+  if (!output(a[4], a[5], shape, dev, &out, &type)) Py_RETURN_NONE;
   const auto fn = mode == 0 ? hb_grouped_gemm : (mode == 1 ? hb_grouped_gemm_dx : hb_grouped_gemm_dw);
-  const int rc = fn(x->const_data_ptr(), w->const_data_ptr(), out.mutable_data_ptr(), offsets_ptr(off),
-                    static_cast<int>(T), static_cast<int>(K), static_cast<int>(N), static_cast<int>(E),
-                    static_cast<hb_dtype>(in), static_cast<hb_dtype>(code_of(out.scalar_type())), nullptr, stream_of(dev));
+  int rc;
+  {
+    Unlocked unlocked;
+    allocate(&out, shape, *x, type);
+    rc = fn(x->const_data_ptr(), w->const_data_ptr(), out.mutable_data_ptr(), offsets_ptr(off), static_cast<int>(T),
+            static_cast<int>(K), static_cast<int>(N), static_cast<int>(E), static_cast<hb_dtype>(in),
+            static_cast<hb_dtype>(code_of(type)), nullptr, stream_of(dev));
+  }
   return answer(rc, a[4], out);
   END_HANDLE_TH_ERRORS
 }
@@ -146,28 +168,29 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (in < 0 || !mx_shape(*x, K, off, &m)) Py_RETURN_NONE;
   const int dev = device_of({x, off ? off : x});
   if (dev < 0) Py_RETURN_NONE;
-  const int64_t code_shape[3] = {x->size(0), dim == 3 ? x->size(1) : K / 2, K / 2};
-  const int64_t scale_shape[2] = {dim == 3 ? m.batch : static_cast<int64_t>(m.bytes), static_cast<int64_t>(m.bytes)};
-  const auto bytes = x->options().dtype(at::kByte).requires_grad(false);
+  const int64_t code_sizes[3] = {x->size(0), dim == 3 ? x->size(1) : K / 2, K / 2};
+  const int64_t scale_sizes[2] = {dim == 3 ? m.batch : static_cast<int64_t>(m.bytes), static_cast<int64_t>(m.bytes)};
+  const at::IntArrayRef code_shape(code_sizes, dim), scale_shape(scale_sizes, dim - 1);
   at::Tensor codes, scales;
-  if (a[2] == Py_None) {
-    codes = at::empty(at::IntArrayRef(code_shape, dim), bytes);
-  } else {
+  if (a[2] != Py_None) {
     const at::Tensor* t = dense(a[2]);
-    if (!is_u8(t, dim) || t->sizes() != at::IntArrayRef(code_shape, dim) || t->get_device() != dev) Py_RETURN_NONE;
+    if (!is_u8(t, dim) || t->sizes() != code_shape || t->get_device() != dev) Py_RETURN_NONE;
     codes = *t;
   }
-  if (a[3] == Py_None) {
-    scales = at::empty(at::IntArrayRef(scale_shape, dim - 1), bytes);
-  } else {
+  if (a[3] != Py_None) {
     const at::Tensor* t = dense(a[3]);
     if (!t || !scales_fit(*t, m, dim) || t->get_device() != dev) Py_RETURN_NONE;
     scales = *t;
   }
-  const int rc = hb_quantize_mxfp4(x->const_data_ptr(), codes.mutable_data_ptr(), scales.mutable_data_ptr(),
-                                   off ? offsets_ptr(off) : nullptr, static_cast<int>(m.batch), static_cast<int>(m.rows),
-                                   static_cast<int>(K), static_cast<int>(m.groups), static_cast<hb_dtype>(in),
-                                   stream_of(dev));
+  int rc;
+  {
+    Unlocked unlocked;
+    allocate(&codes, code_shape, *x, at::kByte);
+    allocate(&scales, scale_shape, *x, at::kByte);
+    rc = hb_quantize_mxfp4(x->const_data_ptr(), codes.mutable_data_ptr(), scales.mutable_data_ptr(),
+                           off ? offsets_ptr(off) : nullptr, static_cast<int>(m.batch), static_cast<int>(m.rows),
+                           static_cast<int>(K), static_cast<int>(m.groups), static_cast<hb_dtype>(in), stream_of(dev));
+  }
   if (rc != HB_OK) return PyLong_FromLong(rc);
   PyObject* pair = PyTuple_New(2);
   if (!pair) return nullptr;
@@ -192,13 +215,20 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!mx_shape(*codes, K, off, &m) || !scales_fit(*scales, m, dim)) Py_RETURN_NONE;
   const int dev = device_of({codes, scales, off ? off : codes});
   if (dev < 0) Py_RETURN_NONE;
-  const int64_t shape[3] = {codes->size(0), dim == 3 ? codes->size(1) : K, K};
+  const int64_t sizes[3] = {codes->size(0), dim == 3 ? codes->size(1) : K, K};
+  const at::IntArrayRef shape(sizes, dim);
   at::Tensor out;
-  if (!output(a[3], a[4], at::IntArrayRef(shape, dim), *codes, &out) || out.get_device() != dev) Py_RETURN_NONE;
-  const int rc = hb_dequantize_mxfp4(codes->const_data_ptr(), scales->const_data_ptr(), out.mutable_data_ptr(),
-                                     off ? offsets_ptr(off) : nullptr, static_cast<int>(m.batch),
-                                     static_cast<int>(m.rows), static_cast<int>(K), static_cast<int>(m.groups),
-                                     static_cast<hb_dtype>(code_of(out.scalar_type())), stream_of(dev));
+  at::ScalarType type;
+  if (!output(a[3], a[4], shape, dev, &out, &type)) Py_RETURN_NONE;
+  int rc;
+  {
+    Unlocked unlocked;
+    allocate(&out, shape, *codes, type);
+    rc = hb_dequantize_mxfp4(codes->const_data_ptr(), scales->const_data_ptr(), out.mutable_data_ptr(),
+                             off ? offsets_ptr(off) : nullptr, static_cast<int>(m.batch), static_cast<int>(m.rows),
+                             static_cast<int>(K), static_cast<int>(m.groups), static_cast<hb_dtype>(code_of(type)),
+                             stream_of(dev));
+  }
   return answer(rc, a[3], out);
   END_HANDLE_TH_ERRORS
 }
@@ -219,14 +249,20 @@ PyObject* mx(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (dev < 0) Py_RETURN_NONE;
   const int64_t shape[2] = {mx_.rows, mw.rows};
   at::Tensor out;
-  if (!output(a[5], a[6], shape, *x, &out) || out.get_device() != dev) Py_RETURN_NONE;
-  const hb_dtype ot = static_cast<hb_dtype>(code_of(out.scalar_type()));
+  at::ScalarType type;
+  if (!output(a[5], a[6], shape, dev, &out, &type)) Py_RETURN_NONE;
+  const hb_dtype ot = static_cast<hb_dtype>(code_of(type));
   const int T = static_cast<int>(mx_.rows), N = static_cast<int>(mw.rows), k = static_cast<int>(K);
-  const int rc = off ? hb_grouped_gemm_mxfp4(x->const_data_ptr(), xs->const_data_ptr(), w->const_data_ptr(),
-                                             ws->const_data_ptr(), out.mutable_data_ptr(), offsets_ptr(off), T, k, N,
-                                             static_cast<int>(mw.batch), ot, nullptr, stream_of(dev))
-                     : hb_gemm_mxfp4(x->const_data_ptr(), xs->const_data_ptr(), w->const_data_ptr(),
-                                     ws->const_data_ptr(), out.mutable_data_ptr(), T, k, N, ot, nullptr, stream_of(dev));
+  int rc;
+  {
+    Unlocked unlocked;
+    allocate(&out, shape, *x, type);
+    rc = off ? hb_grouped_gemm_mxfp4(x->const_data_ptr(), xs->const_data_ptr(), w->const_data_ptr(), ws->const_data_ptr(),
+                                     out.mutable_data_ptr(), offsets_ptr(off), T, k, N, static_cast<int>(mw.batch), ot,
+                                     nullptr, stream_of(dev))
+             : hb_gemm_mxfp4(x->const_data_ptr(), xs->const_data_ptr(), w->const_data_ptr(), ws->const_data_ptr(),
+                             out.mutable_data_ptr(), T, k, N, ot, nullptr, stream_of(dev));
+  }
   return answer(rc, a[5], out);
   END_HANDLE_TH_ERRORS
 }

@@ -295,3 +295,41 @@ def test_overlapping_offsets(K, knobs):
                 free[s:t] = False
             assert near[~free].all(), "%s %s: rows %s" % (fn.__name__, off, (~near.all(1) & ~free).nonzero().flatten().tolist())
             assert (out[free] == 7.0).all()
+
+
+def test_other_threads_run_while_a_launch_waits(K):
+    """Launches behind a long kernel fill the stream's queue until one of them has to wait; Python's lock is free
+    meanwhile.  (A host function in that queue that needs the lock would otherwise wait for good.)"""
+    import threading
+    import time
+    x, w, dy, _, offsets = make(1, [2, 2], 0, 0, 64, 64, torch.float16)
+    out = torch.empty(4, 64, device="cuda")
+    codes, scales = K.quantize_mxfp4(x)
+    wq = K.quantize_mxfp4(w[0])
+    calls = [lambda: K.grouped_gemm(x, w, offsets, out=out), lambda: K.quantize_mxfp4(x, codes=codes, scales=scales),
+             lambda: K.dequantize_mxfp4(codes, scales, out=out), lambda: K.gemm_mxfp4(codes, scales, *wq, out=out)]
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        gaps, stop = [0.0], threading.Event()
+
+        def watch():
+            last = time.perf_counter()
+            while not stop.is_set():
+                time.sleep(0.001)
+                now = time.perf_counter()
+                gaps.append(now - last)
+                last = now
+        thread = threading.Thread(target=watch)
+        thread.start()
+        torch.cuda._sleep(800_000_000)  # 0.4 s
+        longest = 0.0
+        for _ in range(3000):
+            t0 = time.perf_counter()
+            call()
+            longest = max(longest, time.perf_counter() - t0)
+        stop.set()
+        thread.join()
+        torch.cuda.synchronize()
+        assert longest > 0.1, "no launch had to wait: the test shows nothing"
+        assert max(gaps) < longest / 2
