@@ -591,7 +591,10 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const long long row0 = MODE == kDw ? tl.c0 : static_cast<long long>(tl.start) + tl.c0;
       const long long first = (MODE == kDw ? tl.e * p.out_group : 0) + row0 * p.ldc + m;
       if (!empty) {
-        if (!mbar_wait_relaxed(smem_u32(&bars->tmem_full[acc]), acc_phase, wctx)) break;
+        // (a whole reduction's wait, its bound by the blocks: 2^24 of them, the most there are, take 4.3 s, and what goes
+        // wrong in one ends at the ring's waits)
+        const WaitCtx whole{abort_flag, wctx.limit_cycles + (tl.kb1 - tl.kb0) * 8192LL};
+        if (!mbar_wait_relaxed(smem_u32(&bars->tmem_full[acc]), acc_phase, whole)) break;
         tc_fence_after();
       }
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * p.BN);
