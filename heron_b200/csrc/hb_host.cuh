@@ -38,9 +38,12 @@ typedef CUresult (*EncodeIm2colFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapSwizzle, CUtensorMapL2promotion,
                                    CUtensorMapFloatOOBfill);
 
+typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
+
 struct Driver {
   EncodeTiledFn tiled = nullptr;
   EncodeIm2colFn im2col = nullptr;
+  CtxGetCurrentFn context = nullptr;
   int sm_count = 0;
   int driver_version = 0;
   int status = HB_ERR_DEVICE;
@@ -113,6 +116,14 @@ bool setup_device(Driver* d) {
   return true;
 }
 
+// The device's context current in this thread, for the tensor maps' encoders: they are driver calls, which do not bring
+// it along as the runtime's do, and a thread that has called neither (autograd's, a server's worker) has none.
+void bind_context(const Driver& d, int dev) {
+  CUcontext context = nullptr;
+  if (d.context(&context) == CUDA_SUCCESS && context) return;
+  if (cudaSetDevice(dev) != cudaSuccess) cudaGetLastError();  // (what follows then reports it)
+}
+
 Driver& driver() {
   static Driver per_device[kMaxDev];
   static bool tried[kMaxDev] = {false};
@@ -125,7 +136,10 @@ Driver& driver() {
   }
   std::lock_guard<std::mutex> lock(mu);
   Driver& d = per_device[dev];
-  if (tried[dev]) return d;
+  if (tried[dev]) {
+    if (d.status == HB_OK) bind_context(d, dev);
+    return d;
+  }
   tried[dev] = true;
   if (!setup_device(&d)) {
     cudaGetLastError();
@@ -143,6 +157,12 @@ Driver& driver() {
       q != cudaDriverEntryPointSuccess || fn == nullptr)
     return d;
   d.im2col = reinterpret_cast<EncodeIm2colFn>(fn);
+  fn = nullptr;
+  if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+      q != cudaDriverEntryPointSuccess || fn == nullptr)
+    return d;
+  d.context = reinterpret_cast<CtxGetCurrentFn>(fn);
+  bind_context(d, dev);
   d.status = HB_OK;
   return d;
 }
