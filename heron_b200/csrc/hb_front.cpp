@@ -10,6 +10,7 @@
 //
 // Every function returns the result, an int (a status of the library that is not HB_OK), or None.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -37,6 +38,9 @@ const at::Tensor* dense(PyObject* o) {
 }
 
 bool is_u8(const at::Tensor* t, int dim) { return t && t->dim() == dim && t->scalar_type() == at::kByte; }
+
+// Whether a caller would expect a graph behind the output (the other path refuses that).
+bool wants_graph(const at::Tensor* t) { return t && t->requires_grad() && c10::GradMode::is_enabled(); }
 
 // Sizes as the library takes them; false beyond its ints.
 bool fits(int64_t v) { return v >= 0 && v <= 0x7fffffff; }
@@ -97,7 +101,7 @@ PyObject* grouped(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const long mode = PyLong_AsLong(a[0]);
   const at::Tensor *x = dense(a[1]), *w = dense(a[2]), *off = dense(a[3]);
   if (!x || !w || !off || x->dim() != 2 || w->dim() != (mode == 2 ? 2 : 3) || x->scalar_type() != w->scalar_type() ||
-      off->dim() != 1 || off->scalar_type() != at::kInt || off->numel() < 2)
+      off->dim() != 1 || off->scalar_type() != at::kInt || off->numel() < 2 || wants_graph(x) || wants_graph(w))
     Py_RETURN_NONE;
   const int in = code_of(x->scalar_type());
   if (in < 0) Py_RETURN_NONE;
@@ -119,7 +123,7 @@ PyObject* grouped(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::ScalarType type;
   const int64_t sizes[3] = {mode == 2 ? E : T, mode == 1 ? K : N, K};
   const at::IntArrayRef shape(sizes, mode == 2 ? 3 : 2);
-  if (!output(a[4], a[5], shape, dev, &out, &type)) Py_RETURN_NONE;
+  if (!output(a[4], a[5], shape, dev, &out, &type) || (out.defined() && wants_graph(&out))) Py_RETURN_NONE;
   const auto fn = mode == 0 ? hb_grouped_gemm : (mode == 1 ? hb_grouped_gemm_dx : hb_grouped_gemm_dw);
   int rc;
   {

@@ -617,6 +617,14 @@ def _fits(sizes):
         raise _lib.HeronB200Error(_lib.HB_ERR_SHAPE, "sizes %s" % (sizes,))
 
 
+def _no_graph(kind, *tensors):
+    """The products are called outside autograd: an output without a graph would end training in silence."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("%s builds no autograd graph, and one of its tensors requires a gradient: call it under "
+                         "torch.no_grad() or in an autograd.Function (with its gradient operators), or detach"
+                         % kind.replace("hb_", "", 1))
+
+
 def _groups(offsets, groups=None):
     n = offsets.numel() - 1
     if offsets.dim() != 1 or n < 1 or (groups is not None and n != groups):
@@ -641,6 +649,7 @@ def _result(out, shape, like, out_dtype):
 
 def _grouped_args(kind, first, second, offsets, out, out_dtype):
     """(tensors in ABI order, sizes T, K, N, E and types) of one of the three grouped products."""
+    _no_graph(kind, first, second, out)
     if kind == "hb_grouped_gemm_dw":
         T, N = _dims(first, "dy", 2)
         T2, K = _dims(second, "x", 2)
@@ -684,7 +693,11 @@ def grouped_gemm(x, w, offsets, out=None, out_dtype=None, knobs=None):
     Group e owns rows offsets[e] .. offsets[e+1]-1 (offsets: int32 on the device, E + 1 entries; it is
     read by the kernel, so a captured call may be replayed with other offsets).  float16 or bfloat16
     operands, fp32 accumulation, out float32 (default), float16 or bfloat16.  K % 8 == 0.  Rows of no
-    group are left as they are in `out` (arbitrary in a fresh one)."""
+    group are left as they are in `out` (arbitrary in a fresh one).
+
+    No autograd graph is built: under torch.enable_grad() tensors that require a gradient are refused, here and
+    in the two gradients.  An autograd.Function calls this in its forward and grouped_gemm_dx and
+    grouped_gemm_dw in its backward."""
     if knobs is None:
         done = _fast.grouped(0, x, w, offsets, out, out_dtype)
         if done is not None:

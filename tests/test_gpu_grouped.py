@@ -333,3 +333,36 @@ def test_other_threads_run_while_a_launch_waits(K):
         torch.cuda.synchronize()
         assert longest > 0.1, "no launch had to wait: the test shows nothing"
         assert max(gaps) < longest / 2
+
+
+def test_tensors_that_require_a_gradient(K):
+    """Refused where a graph would be expected; in an autograd.Function the operators are its forward and backward."""
+    x, w, dy, off, offsets = make(2, [20, 0, 44], 0, 0, 64, 128, torch.float16)
+    x.requires_grad_()
+    w.requires_grad_()
+    for call in (lambda: K.grouped_gemm(x, w, offsets), lambda: K.grouped_gemm(x.detach(), w, offsets),
+                 lambda: K.grouped_gemm(x, w.detach(), offsets), lambda: K.grouped_gemm_dx(dy, w, offsets),
+                 lambda: K.grouped_gemm_dw(dy, x, offsets),
+                 lambda: K.grouped_gemm(x.detach(), w.detach(), offsets, out=torch.empty(64, 128, device="cuda").requires_grad_())):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+
+    class Experts(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            ctx.save_for_backward(x, w)
+            return K.grouped_gemm(x, w, offsets, out_dtype=x.dtype)
+
+        @staticmethod
+        def backward(ctx, dy):
+            x, w = ctx.saved_tensors
+            dy = dy.contiguous()
+            return K.grouped_gemm_dx(dy, w, offsets, out_dtype=x.dtype), K.grouped_gemm_dw(dy, x, offsets, out_dtype=w.dtype)
+    y = Experts.apply(x, w)
+    y.backward(dy)
+    want, mag, _ = grouped(x.detach(), w.detach(), off)
+    assert_product(y.detach(), want, mag, 64)
+    want, mag, _ = grouped(dy, w.detach().transpose(1, 2), off)
+    assert_product(x.grad, want, mag, 128)
+    want, mag = grouped_dw(dy, x.detach(), off, 3)
+    assert_product(w.grad, want, mag, 44)

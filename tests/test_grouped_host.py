@@ -223,3 +223,27 @@ def test_the_definition_of_the_format():
     assert byte.item() == 127  # largest magnitude in [4, 8): scale 1
     assert values[0, :16].tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, -0.5, -0.5, 0.5, 4.0, 6.0, -4.0, 6.0, 0.0]
     assert [GRID[int(c) & 7] for c in code[0, :8]] == values[0, :8].abs().tolist()
+
+
+def test_tensors_that_require_a_gradient_are_refused(hb_lib):
+    """No output without a graph in silence; without grad mode (an autograd.Function's forward) the call goes on to
+    the next check."""
+    from heron_b200 import kernels as K
+    x, w = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(2, 64, 64, dtype=torch.float16)
+    off, out = torch.zeros(3, dtype=torch.int32), torch.zeros(4, 64)
+    xg, wg, og = (t.clone().requires_grad_() for t in (x, w, out))
+    calls = [lambda x, w, out: K.grouped_gemm(x, w, off, out=out), lambda x, w, out: K.grouped_gemm_dx(x, w, off, out=out),
+             lambda x, w, out: K.plan_grouped_gemm(x, w, off, out=out), lambda x, w, out: K.plan_grouped_gemm_dx(x, w, off, out=out),
+             lambda x, w, out: K.grouped_gemm(x, w, off, out=out, knobs=dict(tile_n=64))]
+    for call in calls:
+        for bad in ((xg, w, None), (x, wg, None), (x, w, og)):
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call(*bad)
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+                call(*bad)
+        with pytest.raises(ValueError, match="CUDA"):
+            call(xg.detach(), w, out)
+    for fn in (K.grouped_gemm_dw, K.plan_grouped_gemm_dw):
+        for a, b in ((xg, x), (x, xg)):
+            with pytest.raises(ValueError, match="requires a gradient"):
+                fn(a, b, off)
