@@ -2,11 +2,14 @@
 
     python -m heron_b200.build [--force] [--verbose]
 
-The library is the package's only compute path.  nvcc cross-compiles without a GPU.
+The library is the package's only compute path.  nvcc cross-compiles without a GPU.  Where torch can be
+imported, the C++ front end of some of its operators is built beside it; a host of the C ABI needs neither.
 """
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -14,7 +17,7 @@ TARGET = os.path.join(HERE, "libheron_b200.so")
 SOURCES = [os.path.join(CSRC, "hb_api.cu")]
 HEADER = os.path.join(HERE, os.pardir, "include", "heron_b200.h")
 # the C++ front end of the grouped and 4-bit operators (a CPython extension next to the library)
-FRONT = os.path.join(HERE, "_front.so")
+FRONT = os.path.join(HERE, "_front" + sysconfig.get_config_var("EXT_SUFFIX"))
 FRONT_SOURCE = os.path.join(CSRC, "hb_front.cpp")
 
 
@@ -58,26 +61,52 @@ def _run(cmd, target, verbose):
             os.remove(tmp)
 
 
+def cuda_include():
+    """The headers of the toolkit that nvcc() belongs to."""
+    cc = nvcc()
+    return os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(cc) or cc))), "include")
+
+
+def front_key():
+    """What the front end is built for: it links torch's C++ library, which promises no stable interface.  The extension
+    carries it as `built_for`, and another one is neither taken for up to date nor called."""
+    import torch
+    return "heron_b200 front end for torch %s" % torch.__version__
+
+
+def front_is_stale():
+    if not os.path.exists(FRONT):
+        return True
+    t = os.path.getmtime(FRONT)
+    if any(os.path.getmtime(s) > t for s in (FRONT_SOURCE, HEADER, os.path.abspath(__file__))):
+        return True
+    with open(FRONT, "rb") as f:
+        return front_key().encode() + b"\0" not in f.read()
+
+
 def build_front(force=False, verbose=False):
-    """heron_b200/_front.so, linked against the library beside it and torch's own libraries."""
-    sources = (FRONT_SOURCE, HEADER, os.path.abspath(__file__))
-    if not force and os.path.exists(FRONT) and all(os.path.getmtime(s) <= os.path.getmtime(FRONT) for s in sources):
+    """The front end, linked against the library beside it and torch's own libraries."""
+    if not force and not front_is_stale():
         return FRONT
-    import sysconfig
     import torch
     from torch.utils import cpp_extension
-    inc = cpp_extension.include_paths() + ["/usr/local/cuda/include", sysconfig.get_paths()["include"]]
+    inc = cpp_extension.include_paths() + [cuda_include(), sysconfig.get_paths()["include"]]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+          '-DHB_FRONT_KEY="%s"' % front_key()]
          + [f for i in inc for f in ("-isystem", i)] + [FRONT_SOURCE, "-L" + HERE, "-l:libheron_b200.so", "-L" + lib,
          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], FRONT, verbose)
     return FRONT
 
 
 def build(force=False, verbose=False, extra_flags=()):
-    """Builds what is out of date and returns the library's path."""
+    """Builds what is out of date and returns the library's path.  The front end is left out, with a word on stderr, where
+    torch, its headers or a C++ compiler are missing: kernels.py does its work without it."""
     build_library(force, verbose, extra_flags)
-    build_front(force, verbose)
+    try:
+        build_front(force, verbose)
+    except (ImportError, OSError, subprocess.CalledProcessError) as e:
+        print("heron_b200: front end not built (%s: %s)" % (type(e).__name__, e), file=sys.stderr)
     return TARGET
 
 

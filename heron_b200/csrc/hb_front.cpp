@@ -277,4 +277,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__front(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__front(void) {
+  PyObject* m = PyModule_Create(&module);
+  // (the torch that this is built for, see build.py)
+  if (m && PyModule_AddStringConstant(m, "built_for", HB_FRONT_KEY) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

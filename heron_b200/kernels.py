@@ -6,6 +6,7 @@ the reference operators' own: GEMM / batched GEMM take ``B`` as (N, K) (ops/cuda
 ops/cuda/batch_matmul.py:8), NHWC conv takes an HWIO filter (ops/cuda/conv2d.py:155).
 """
 import ctypes
+import warnings
 
 import torch
 
@@ -545,20 +546,29 @@ _WIDE_CODES = {torch.float16: _lib.HB_F16, torch.bfloat16: _lib.HB_BF16, torch.f
 # The small calls of these operators are bound by the host (a token's product takes the GPU a few
 # microseconds).  A call without knobs first goes to the C++ front end (csrc/hb_front.cpp), which checks,
 # allocates and launches in one step; what it finds unusual it hands back (None), and the code below
-# checks again, names the fault or does the call.
+# checks again, names the fault or does the call.  Without the extension it does every call, at some
+# 6 us more of the host's time each.
 class _Front:
     """The extension module, loaded by the first call (importing this file loads nothing)."""
 
+    NAMES = ("grouped", "quantize", "dequantize", "mx")
+
     def __getattr__(self, name):
+        if name not in self.NAMES:
+            raise AttributeError(name)
         _lib.load()
+        from . import build
         try:
             from . import _front
+            if getattr(_front, "built_for", None) != build.front_key():
+                raise ImportError("it is built for another torch")
         except ImportError as e:
-            raise ImportError("heron_b200/_front.so is not built or does not load (run `python -m "
-                              "heron_b200.build`): %s" % e)
-        for fn in ("grouped", "quantize", "dequantize", "mx"):
-            setattr(self, fn, getattr(_front, fn))
-        return getattr(_front, name)
+            warnings.warn("heron_b200: no C++ front end, calls take longer on the host (run `python -m heron_b200.build`): %s"
+                          % e, RuntimeWarning, stacklevel=3)
+            _front = None
+        for fn in self.NAMES:
+            setattr(self, fn, getattr(_front, fn) if _front else lambda *args: None)
+        return getattr(self, name)
 
 
 _fast = _Front()

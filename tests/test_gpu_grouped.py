@@ -366,3 +366,24 @@ def test_tensors_that_require_a_gradient(K):
     assert_product(x.grad, want, mag, 128)
     want, mag = grouped_dw(dy, x.detach(), off, 3)
     assert_product(w.grad, want, mag, 44)
+
+
+def test_without_the_front_end(K, monkeypatch):
+    """The Python path does the same calls."""
+    from heron_b200._lib import HeronB200Error
+    x, w, dy, off, offsets = make(2, [20, 0, 44], 0, 0, 64, 128, torch.float16)
+
+    def all_calls():
+        xq, wq = K.quantize_mxfp4(x, offsets=offsets), K.quantize_mxfp4(w)
+        aq, bq = K.quantize_mxfp4(x), K.quantize_mxfp4(w[0])
+        return [K.grouped_gemm(x, w, offsets), K.grouped_gemm_dx(dy, w, offsets), K.grouped_gemm_dw(dy, x, offsets),
+                K.grouped_gemm_mxfp4(*xq, *wq, offsets), K.gemm_mxfp4(*aq, *bq), K.dequantize_mxfp4(*wq)]
+    want = all_calls()
+    front = K._Front()
+    for name in front.NAMES:
+        setattr(front, name, lambda *args: None)
+    monkeypatch.setattr(K, "_fast", front)
+    for got, ref in zip(all_calls(), want):
+        assert torch.equal(got, ref)
+    with pytest.raises(HeronB200Error):
+        K.grouped_gemm(x, w.bfloat16(), offsets)

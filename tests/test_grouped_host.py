@@ -247,3 +247,60 @@ def test_tensors_that_require_a_gradient_are_refused(hb_lib):
         for a, b in ((xg, x), (x, xg)):
             with pytest.raises(ValueError, match="requires a gradient"):
                 fn(a, b, off)
+
+
+def test_a_call_without_the_front_end_takes_the_python_path(hb_lib, monkeypatch):
+    """An extension that is missing, or built for another torch, costs a warning and no call."""
+    import sys
+    import types
+    import heron_b200
+    from heron_b200 import kernels as K
+    x, w, off = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(2, 8, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32)
+
+    def never(*args):
+        raise AssertionError("called")
+    other = types.SimpleNamespace(built_for="another", grouped=never, quantize=never, dequantize=never, mx=never)
+    for module in (None, other, types.SimpleNamespace(**dict(vars(other), built_for=None))):
+        monkeypatch.setitem(sys.modules, "heron_b200._front", module)
+        monkeypatch.setattr(heron_b200, "_front", module, raising=False)
+        if module is None:
+            monkeypatch.delattr(heron_b200, "_front")
+        monkeypatch.setattr(K, "_fast", K._Front())
+        with pytest.warns(RuntimeWarning, match="front end"), pytest.raises(ValueError, match="CUDA"):
+            K.grouped_gemm(x, w, off)
+        with pytest.raises(ValueError, match="CUDA"):
+            K.quantize_mxfp4(x)
+
+
+def test_the_library_builds_without_torch(hb_lib, monkeypatch, capsys):
+    import os
+    import subprocess
+    import sys
+    from heron_b200 import build
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build() == build.TARGET
+    assert "front end not built" in capsys.readouterr().err
+    # as a command, from nothing but the package's own files
+    code = "import sys; sys.modules['torch'] = None; from heron_b200 import build; assert build.build() == build.TARGET"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(build.__file__)))
+    assert subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True).returncode == 0
+
+
+def test_the_front_end_follows_torch_and_the_toolkit(hb_lib, monkeypatch, tmp_path):
+    import os
+    from heron_b200 import build
+    assert build.FRONT.endswith(build.sysconfig.get_config_var("EXT_SUFFIX"))
+    assert not build.front_is_stale()
+    nvcc = tmp_path / "bin" / "nvcc"
+    nvcc.parent.mkdir()
+    nvcc.write_text("")
+    with monkeypatch.context() as m:
+        m.setenv("NVCC", str(nvcc))
+        assert build.cuda_include() == os.path.realpath(tmp_path / "include")
+    commands = []
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "9.9.9")
+        m.setattr(build, "_run", lambda cmd, target, verbose: commands.append((cmd, target)))
+        assert build.front_is_stale()
+        build.build_front()
+    assert len(commands) == 1 and commands[0][1] == build.FRONT and any("9.9.9" in c for c in commands[0][0])
