@@ -387,3 +387,28 @@ def test_without_the_front_end(K, monkeypatch):
         assert torch.equal(got, ref)
     with pytest.raises(HeronB200Error):
         K.grouped_gemm(x, w.bfloat16(), offsets)
+
+
+NARROW = {"few": [1, 2, 3, 2] * 10, "uneven": [0, 1, 40, 3, 64, 0, 33, 5] * 5, "long_runs": [0] * 8 + [70] * 32}
+
+
+@pytest.mark.parametrize("counts", list(NARROW))
+@pytest.mark.parametrize("m,r", [(2048, 64), (2040, 200), (2048, 520)])
+@pytest.mark.parametrize("od", [torch.float32, torch.bfloat16])
+def test_narrow_tiles_in_several_rounds(K, counts, m, r, od):
+    """More tiles than two CTAs on every SM take at once: rings and accumulators go round from tile to tile."""
+    c = NARROW[counts]
+    x, w, _, off, offsets = make(m + r, c, 1, 2, r, m, torch.bfloat16)
+    out = torch.full((x.shape[0], m), 7.0, dtype=od, device="cuda")
+    plan = K.plan_grouped_gemm(x, w, offsets, out=out)
+    if counts != "long_runs":  # (long runs: about 50 rows a group and more take wider tiles)
+        assert plan.knobs()["tile_n"] == 64 and plan.knobs()["grid"] > K._lib.load().hb_sm_count()
+    plan.launch()
+    want, mag, own = grouped(clean(x), w, off)
+    assert_product(out[own], want[own], mag[own], r, "y")
+    assert (out[~own] == 7.0).all()
+    dy, wt = x, w.transpose(1, 2).contiguous()  # (rows of r values, weights (E, r, m): dx has m features)
+    out.fill_(7.0)
+    K.grouped_gemm_dx(dy, wt, offsets, out=out)
+    assert_product(out[own], want[own], mag[own], r, "dx")
+    assert (out[~own] == 7.0).all()

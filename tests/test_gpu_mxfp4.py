@@ -390,3 +390,51 @@ def test_overlapping_offsets(K, k):
             want, mag, _ = grouped(xv, wv, off)
             assert_product(out[once], want[once], mag[once], k, "%s %s" % (off, knobs))
             assert (out[(owners == 0).cuda()] == 7.0).all()
+
+
+def grouped_operands(K, counts, lead, tail, k, n):
+    off = offsets_of(counts, lead)
+    offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+    T = off[-1] + tail
+    x, w = randn(4, T, k, dtype=torch.bfloat16), randn(5, len(counts), n, k, dtype=torch.bfloat16)
+    xq, wq = K.quantize_mxfp4(x, offsets=offsets), K.quantize_mxfp4(w)
+    xv = torch.zeros(T, k, device="cuda")
+    K.dequantize_mxfp4(*xq, offsets=offsets, out=xv)
+    return off, offsets, xq, wq, grouped(xv, K.dequantize_mxfp4(*wq), off)
+
+
+@pytest.mark.parametrize("counts", [[1, 2, 3, 2] * 8, [0, 1, 40, 3, 64, 0, 33, 5] * 4, [129] * 6 + [0] * 26])
+@pytest.mark.parametrize("k,n", [(416, 2048), (1024, 2000)])
+def test_grouped_product_in_several_rounds(K, counts, k, n):
+    """More tiles than the CTAs that run at once, the default's choice of tiles."""
+    off, offsets, xq, wq, (want, mag, own) = grouped_operands(K, counts, 1, 2, k, n)
+    for od in (torch.float32, torch.bfloat16):
+        out = torch.full(want.shape, 7.0, dtype=od, device="cuda")
+        K.grouped_gemm_mxfp4(*xq, *wq, offsets, out=out)
+        assert_product(out[own], want[own], mag[own], k)
+        assert (out[~own] == 7.0).all()
+
+
+@pytest.mark.parametrize("counts,lead,tail", [([3, 0, 1, 4], 0, 0), ([3, 0, 1, 2], 1, 1), ([0, 8], 0, 0), ([9, 0, 0, 1, 17], 3, 0),
+                                              ([1] * 20, 130, 0)])
+@pytest.mark.parametrize("k,n", [(416, 300), (64, 130), (1056, 17)])
+def test_few_rows_of_several_groups(K, counts, lead, tail, k, n):
+    """The kernel of few rows with more than one tile of scales to an expert and groups that start inside a tile."""
+    off, offsets, xq, wq, (want, mag, own) = grouped_operands(K, counts, lead, tail, k, n)
+    for knobs in (None, dict(tile_n=64)):
+        out = torch.full(want.shape, 7.0, device="cuda")
+        K.grouped_gemm_mxfp4(*xq, *wq, offsets, out=out, knobs=knobs)
+        assert_product(out[own], want[own], mag[own], k, str(knobs))
+        assert (out[~own] == 7.0).all()
+
+
+@pytest.mark.parametrize("split", [2, 4, 8])
+@pytest.mark.parametrize("counts", [[0, 1, 0, 2, 70], [17, 0, 128, 1, 129, 63], [0, 0]])
+@pytest.mark.parametrize("k,n", [(96, 130), (2080, 300)])
+def test_grouped_reduction_over_a_cluster(K, split, counts, k, n):
+    off, offsets, xq, wq, (want, mag, own) = grouped_operands(K, counts, 2, 3, k, n)
+    for extra in (dict(), dict(max_ctas=2 * split), dict(stages=1)):
+        out = torch.full(want.shape, 7.0, device="cuda")
+        K.grouped_gemm_mxfp4(*xq, *wq, offsets, out=out, knobs=dict(tile_n=64, split_k=split, **extra))
+        assert_product(out[own], want[own], mag[own], k, str(extra))
+        assert (out[~own] == 7.0).all()
