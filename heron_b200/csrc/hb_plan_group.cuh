@@ -133,24 +133,36 @@ int check_group_knobs(const GroupProblem& g, const hb_knobs& k) {
   return HB_OK;
 }
 
-// Whether a product is left to the kernels that stream the weights (hb_rows.cuh), by the weights that all their
-// passes read: one pass for eight rows of a group, so one for up to eight rows of a single group, and at worst
-// one for every row where there are more groups.  Measured, streaming / tiles (with a cluster or two CTAs to an
-// SM where those are chosen):
-//   bf16, one group: 16.8 million weights in one pass (8 rows, 4096 x 4096) 8.3 / 10.9 us, 67 million (one row) 25.6 /
-//   26.6, but of 8192 and more features, whose tiles fill the SMs, 8 rows 19.2 / 16.7 (K 4096) and one row x 14336 x 4096
-//   27.2 / 21.7; two passes of 16.8 million 15.0 / 11.2, three of 2.1 million (24 rows) 5.3 / 7.6
-//   bf16, rows over 32 experts of 2048 x 2048: 4 rows 6.6 / 9.4, 8 rows 14.5 / 13.7, 16 rows 20.8 / 21.0, 24 rows 27.2 /
-//   27.9 (the memory's time either way); 16 rows over 8 experts 13.9 / 13.0
-//   MXFP4, bound by widening elements: one group, 16.8 million in one pass 6.9 - 8.3 / 8.4, two of 2.1 million 5.2 / 5.8
-//   or (256 x 8192) 11.5 / 8.3; 8.4 million in two or four rows to experts of their own 4.7 and 5.2 / 5.8 and 6.6, 16.8 million 7.7 / 6.4
-// (at most 64 rows: all of them in one group are then eight passes over its weights)
+// Whether a product is left to the kernels that stream the weights (hb_rows.cuh): by the weights that all their passes
+// read (one pass for eight rows of a group, so one for up to eight rows of a single group, and at worst one for every row
+// where there are more groups), and by the blocks that a launch has, T * N / 16, of which those without rows leave at
+// once: with short reductions the blocks' start is the time.  Measured, streaming / tiles of 64 columns (with a cluster or
+// two CTAs to an SM where those are chosen), us, rows x features x reduction; more groups: rows spread at random:
+//   bf16, one group.  Up to 8 rows of 4096 features: K 64 2.2 - 2.9 / 3.1, K 1024 5.7 / 6.5 - 6.8, K 4096 8.3 - 10.3 / 11.2 -
+//   11.5, K 16384 25.4 - 25.9 / 28.0 - 28.5.  64 x 512 x 256 4.5 / 5.8, 16 x 2048 x 2048 6.3 / 7.7.  Between 2^15 and 2^16 rows x
+//   features (8 rows at least): K 1024 8 x 8192 7.2 / 7.6, 32 x 2048 6.4 / 7.8, 64 x 1024 6.8 / 7.5; K 512 6.5 / 5.7, 5.8 /
+//   5.4 (16 x 4096); K 256 32 x 2048 6.0 / 4.8.  Beyond: 1 x 16384 x 512 10.2 / 6.7, 8 x 65536 x 128 44.7 / 6.8, 64 x 2048 x
+//   512 10.4 / 6.8.  More than 8.4 million weights in all passes: 32 x 2048 x 2048 8.5 / 8.2, 24 x 4096 x 2048 11.7 / 9.6
+//   bf16, more groups.  K 2048: 2 rows x 2048 3.7 / 7.8, 4 rows 7.8 / 10.7, 8 rows 11.0 - 14.1 / 11.5 - 12.9, 24 rows over 32
+//   25.6 / 26.5, 48 over 48 44.2 / 41.5 (the memory's time either way).  Shorter ones: 8 x 1024 x 1024 6.0 / 6.8, 10 x 1024 x
+//   1024 6.2 / 7.0, 16 x 512 x 512 5.5 / 5.4, 8 x 2048 x 1024 7.5 - 10.4 / 7.5 - 8.2, 16 x 1024 x 1024 9.2 / 8.1, 32 x 2048 x 256
+//   17.6 / 7.4, 64 x 512 x 512 11.4 / 7.7
+//   MXFP4, bound by widening elements.  One group: 1 row x 4096 x 512 2.6 / 3.8, x 4096 7.5 / 8.8; x 6144 x 2048 6.6 / 6.2,
+//   x 8192 x 1024 5.6 / 5.0, 4 rows 7.0 / 5.0; x 4096 x 8192 12.8 / 10.5; two passes, 16 x 2048 x 1024, 5.5 / 5.0.  More
+//   groups: 4 x 1024 x 1024 3.3 / 4.5, 2 x 2048 x 2048 4.4 / 5.8, 4 x 2048 x 1024 5.6 / 5.0, 8 x 1024 x 512 4.3 / 4.2, 16 x 512 x
+//   512 4.2 / 4.2, 8 x 2048 x 256 6.7 / 4.1, 64 x 512 x 512 11.5 / 5.7; 4 x 2048 x 2048 7.8 / 6.4
 bool few_rows(const GroupProblem& g) {
   if ((g.mode != hb::kFwd && g.mode != hb::kMx) || g.T > 64) return false;
-  const long long weights = static_cast<long long>(g.M) * g.R;
-  if (g.mode == hb::kMx) return g.R <= 8192 && (g.E == 1 ? g.T <= 8 && weights <= (1LL << 24) : g.T * weights <= (1LL << 23));
-  if (g.E == 1) return (g.T <= 8 && g.M <= 4096) || (g.T + 7) / 8 * weights <= (1LL << 23);
-  return g.T <= (g.E > 8 ? g.E : 8);
+  const long long weights = static_cast<long long>(g.M) * g.R, T = g.T;
+  if (g.mode == hb::kMx)
+    return g.R <= 8192 && (g.E == 1 ? T <= 8 && g.M <= 4096 && weights <= (1LL << 24)
+                                    : T * weights <= (1LL << 23) && T * g.M <= 8192);
+  if (g.E == 1) {
+    const long long outputs = (T < 8 ? 8 : T) * g.M;
+    if (outputs > 65536 || (outputs > 32768 && g.R < 1024)) return false;
+    return (T <= 8 && outputs <= 32768) || (T + 7) / 8 * weights <= (1LL << 23);
+  }
+  return T <= (g.E > 8 ? g.E : 8) && (g.R >= 2048 || T * g.M <= 10240);
 }
 
 // Knobs of the tile kernel, given by the caller: then that kernel is meant.

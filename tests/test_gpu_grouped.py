@@ -412,3 +412,49 @@ def test_narrow_tiles_in_several_rounds(K, counts, m, r, od):
     K.grouped_gemm_dx(dy, wt, offsets, out=out)
     assert_product(out[own], want[own], mag[own], r, "dx")
     assert (out[~own] == 7.0).all()
+
+
+@pytest.mark.parametrize("T,E", [(2, 33), (7, 40), (8, 100), (8, 1024)])
+@pytest.mark.parametrize("k,n", [(264, 40), (2056, 17)])
+def test_few_rows_over_many_groups(K, T, E, k, n):
+    """The kernel of few rows with more groups than a warp looks at at once, offsets in order and not."""
+    g = torch.Generator().manual_seed(T + E)
+    x, w, _, _, _ = make(T + k, [T] + [0] * (E - 1), 0, 0, k, n, torch.bfloat16)
+    ordered = torch.randint(0, T + 1, (E + 1,), generator=g).sort().values.tolist()
+    for off in (ordered, torch.randint(-2, T + 3, (E + 1,), generator=g).tolist(), [T] * (E - 1) + [1, T], [0] * E + [T]):
+        offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+        out = torch.full((T, n), 7.0, device="cuda")
+        plan = K.plan_grouped_gemm(x, w, offsets, out=out)
+        assert plan.knobs()["tile_n"] == 0  # the kernel without tiles
+        plan.launch()
+        near = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+        from grouped_util import clamped
+        free = torch.ones(T, dtype=torch.bool, device="cuda")
+        for e, (s, t) in enumerate(clamped(off, T)):
+            if t > s:
+                want, mag, _ = grouped(x[s:t], w[e][None], [0, t - s])
+                near[s:t] |= (out[s:t].double() - want).abs() <= k * 2.0 ** -23 * mag
+                free[s:t] = False
+        assert near[~free].all() and (out[free] == 7.0).all()
+
+
+def test_which_products_stream(K):
+    """The rule of hb_plan_group.cuh, both sides of each border."""
+    def tiles(T, E, n, k):
+        x, w = torch.zeros(T, k, dtype=torch.float16, device="cuda"), torch.zeros(E, n, k, dtype=torch.float16, device="cuda")
+        return K.plan_grouped_gemm(x, w, torch.zeros(E + 1, dtype=torch.int32, device="cuda")).knobs()["tile_n"] > 0
+
+    def mx_tiles(T, E, n, k):
+        kt = -(-k // 128)
+        a, w = (torch.zeros(*s, k // 2, dtype=torch.uint8, device="cuda") for s in ((T,), (E, n)))
+        xs = torch.zeros((T // 128 + E) * kt * 512, dtype=torch.uint8, device="cuda")
+        ws = torch.zeros(E, -(-n // 128) * kt * 512, dtype=torch.uint8, device="cuda")
+        return K.plan_grouped_gemm_mxfp4(a, xs, w, ws, torch.zeros(E + 1, dtype=torch.int32, device="cuda")).knobs()["tile_n"] > 0
+    for T, E, n, k, want in ((8, 1, 4096, 4096, False), (8, 1, 4104, 2048, True), (1, 1, 8192, 1024, False), (1, 1, 8192, 1016, True),
+                             (1, 1, 8200, 64, True), (16, 1, 2048, 2048, False), (32, 1, 2048, 2048, True), (64, 1, 512, 64, False),
+                             (64, 1, 520, 64, True), (65, 1, 64, 64, True), (8, 4, 2048, 2048, False), (8, 4, 1280, 64, False),
+                             (8, 4, 1288, 64, True), (9, 4, 64, 64, True), (10, 12, 64, 64, False), (13, 12, 64, 64, True)):
+        assert tiles(T, E, n, k) == want, (T, E, n, k)
+    for T, E, n, k, want in ((8, 1, 4096, 4096, False), (8, 1, 4128, 64, True), (1, 1, 4096, 4128, True), (9, 1, 64, 64, True),
+                             (4, 4, 2048, 1024, False), (4, 4, 2049, 64, True), (2, 2, 2048, 2080, True), (64, 3, 128, 64, False)):
+        assert mx_tiles(T, E, n, k) == want, (T, E, n, k)
