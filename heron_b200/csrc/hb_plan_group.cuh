@@ -392,7 +392,9 @@ size_t mx_scale_bytes(int batch, int rows, int K, int groups) {
   if (batch <= 0 || rows < 0 || K <= 0 || K % 32 != 0 || groups < 0 || groups > hb::kMaxGroups) return 0;
   if (groups > 0 && batch != 1) return 0;
   const long long tile_rows = groups > 0 ? rows / 128 + groups : (rows + 127LL) / 128;
-  return static_cast<size_t>(batch) * tile_rows * ((K + 127LL) / 128) * hb::kAtomBytes;
+  size_t bytes;  // (one matrix has at most 2^57)
+  return __builtin_mul_overflow(static_cast<size_t>(batch), static_cast<size_t>(tile_rows * ((K + 127LL) / 128) * hb::kAtomBytes), &bytes)
+             ? 0 : bytes;
 }
 
 // Both directions: `values` is the input of the quantisation or the output of the way back.
@@ -406,6 +408,10 @@ int run_mx(bool back, const void* values, const void* codes, const void* scales,
   if (!values || !codes || !scales || !aligned16(values) || !aligned16(codes) || !aligned16(scales)) return HB_ERR_ALIGN;
   if ((groups > 0) != (offsets != nullptr) || (reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) return HB_ERR_ALIGN;
   if (static_cast<long long>(batch) * rows > 0x7fffffffLL) return HB_ERR_SHAPE;
+  // 16 blocks of eight rows to a tile row of scales
+  const long long row_blocks = 16LL * batch * (groups > 0 ? rows / 128 + groups : (rows + 127LL) / 128);
+  const int segments = (K - 1) / hb::kMxSegment + 1;
+  if (segments > 65535 || row_blocks > 0x7fffffffLL) return HB_ERR_SHAPE;
   Driver& d = driver();
   if (d.status != HB_OK) return d.status;
   hb::MxParams p;
@@ -417,10 +423,6 @@ int run_mx(bool back, const void* values, const void* codes, const void* scales,
   p.offsets = offsets;
   p.batch = batch; p.rows = rows; p.K = K; p.groups = groups;
   p.matrix_scales = static_cast<long long>(mx_scale_bytes(1, rows, K, groups));
-  // 16 blocks of eight rows to a tile row of scales
-  const long long row_blocks = 16LL * batch * (groups > 0 ? rows / 128 + groups : (rows + 127LL) / 128);
-  const int segments = (K - 1) / hb::kMxSegment + 1;
-  if (segments > 65535 || row_blocks > 0x7fffffffLL) return HB_ERR_SHAPE;
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(row_blocks), segments);

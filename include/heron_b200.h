@@ -349,7 +349,9 @@ int hb_grouped_gemm_dw(const void* dy, const void* x, void* dw, const int* offse
  * hb_grouped_gemm) and group g's first tile row is offsets[g] / 128 + g; rows of no group are skipped.
  * (Offsets out of order: the groups' tile rows have to rise with g and not to meet, or the rows concerned get
  * arbitrary scales; nothing is read or written out of range.)
- * hb_mxfp4_scale_bytes gives the size of the scale array (0 for sizes the operators refuse).
+ * hb_mxfp4_scale_bytes gives the size of the scale array (0 for no rows without groups, for negative or misaligned
+ * sizes, and where it passes 64 bits).  The two conversions take batch * rows up to 2^31 - 1, K up to 65535 * 1024 and
+ * batch * (rows / 128, rounded up) up to 2^27 - 1; the products their own sizes, below.
  *
  * hb_quantize_mxfp4: in HB_F16, HB_BF16 or HB_F32.  hb_dequantize_mxfp4: the values, out HB_F32,
  * HB_BF16 (both exact) or HB_F16 (rounded; beyond its range infinite).

@@ -304,3 +304,20 @@ def test_the_front_end_follows_torch_and_the_toolkit(hb_lib, monkeypatch, tmp_pa
         assert build.front_is_stale()
         build.build_front()
     assert len(commands) == 1 and commands[0][1] == build.FRONT and any("9.9.9" in c for c in commands[0][0])
+
+
+def test_scale_bytes_that_pass_64_bits(hb_lib):
+    f = hb_lib.hb_mxfp4_scale_bytes
+    one = f(1, 2 ** 31 - 1, 2 ** 31 - 32, 0)
+    assert f(127, 2 ** 31 - 1, 2 ** 31 - 32, 0) == 127 * one
+    assert f(128, 2 ** 31 - 1, 2 ** 31 - 32, 0) == 0 and f(2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 32, 0) == 0
+
+
+def test_largest_conversions(hb_lib, ptrs):
+    """The limits that the header gives are looked at before a device is."""
+    from heron_b200 import _lib
+    _, p, _, _ = ptrs
+    F16 = _lib.HB_F16
+    for fn in (hb_lib.hb_quantize_mxfp4, hb_lib.hb_dequantize_mxfp4):
+        for batch, rows, k in ((1, 4, 65535 * 1024 + 32), (2, 2 ** 30, 32), (2 ** 27, 1, 32)):
+            assert fn(p, p, p, None, batch, rows, k, 0, F16, None) == _lib.HB_ERR_SHAPE
