@@ -263,6 +263,9 @@ int plan_group(const GroupProblem& g, const void* A, const void* B, void* out, c
   plan->grid = static_cast<int>(tiles < units ? tiles : units) * together;
   p.ksplit = k.split_k;
   plan->smem = group_fixed_smem(g.E, k.split_k > 1, narrow) + k.stages * group_stage(g, k.tile_n, k.cta_group);
+  // CTA pairs have their SMs for themselves, also with few stages: of two pairs (of calls on two streams) that share SMs
+  // each could hold the tensor memory of one SM and wait, without a bound, for that of the other.
+  if (k.cta_group == 2 && plan->smem <= kNarrowSmem) plan->smem = kNarrowSmem + 1024;
   plan->knobs = k;
 
   const uint64_t T = g.T, E = g.E, M = g.M, R = g.R, C = g.C;

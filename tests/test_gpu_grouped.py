@@ -458,3 +458,16 @@ def test_which_products_stream(K):
     for T, E, n, k, want in ((8, 1, 4096, 4096, False), (8, 1, 4128, 64, True), (1, 1, 4096, 4128, True), (9, 1, 64, 64, True),
                              (4, 4, 2048, 1024, False), (4, 4, 2049, 64, True), (2, 2, 2048, 2080, True), (64, 3, 128, 64, False)):
         assert mx_tiles(T, E, n, k) == want, (T, E, n, k)
+
+
+@pytest.mark.parametrize("tile_n", [128, 192, 256])
+def test_pairs_do_not_share_an_sm(K, tile_n):
+    """Whatever the stages, two CTAs of pairs need more shared memory than an SM has."""
+    from heron_b200 import kernels
+    x, w, dy, _, offsets = make(2, [300, 20, 44], 0, 0, 64, 128, torch.float16)
+    xq, wq = kernels.quantize_mxfp4(x, offsets=offsets), kernels.quantize_mxfp4(w)
+    for stages in (0, 1, 2, 3):
+        knobs = dict(tile_n=tile_n, cta_group=2, stages=stages)
+        for plan in (K.plan_grouped_gemm(x, w, offsets, knobs=knobs), K.plan_grouped_gemm_dx(dy, w, offsets, knobs=knobs),
+                     K.plan_grouped_gemm_mxfp4(*xq, *wq, offsets, knobs=knobs)):
+            assert 2 * (plan.knobs()["smem_bytes"] + 1024) > 228 * 1024 and plan.knobs()["smem_bytes"] <= 232448
