@@ -39,11 +39,13 @@
 // own features and of all the tile's rows.  SPLIT: the 2, 4 or 8 CTAs of a cluster share a tile's reduction
 // and join their sums through distributed shared memory, in the order of the shares.
 //
-// What bounds it (B200, times in loops of some 10 ms; sustained loops are 15 % slower): 8192 rows over 32 experts of
-// 2048 x 2048 bf16 71 us, 335 MB of traffic at 4.7 TB/s and 57 % of the tensor cycles; dx of 8192 rows, 16 groups of
-// 2048 x 1024 36 us; dw of the same 41 us, where operands into and out of shared memory (48 KB a block each way)
-// take longer than the MMAs; 4096^3 in 4 bits 34.6 us, where a block's scale copies and MMAs take their issuing
-// thread about as long (460 cycles) as the tensor core (512).
+// What bounds it (B200; loops of 0.15 s, in brackets loops of some 10 ms, whose clocks are higher): 8192 rows over 32
+// experts of 2048 x 2048 bf16 88 us (73), 335 MB of traffic at 3.8 TB/s (4.6), tensor cores active 62 %; dx and dw of 8192
+// rows, 16 groups of 2048 x 1024, 96 us (41 + 44): dx has 160 tiles for 74 pairs, 2.2 rounds paid as three; in dw the tensor
+// cores are active 48 % and the operands' path 41 %, and what it waits for is not known (CTA pairs, which halve B's way
+// through shared memory, were level); 4096^3 in 4 bits 39.5 us (34.9): 256 tiles for 74 pairs are 3.46 rounds paid as four,
+// each with one accumulator, and a block's scale copies and MMAs take their issuing thread about as long (460 cycles)
+// as the tensor core (512).
 // Offsets are clamped to [0, T] and a group whose end
 // lies before its start counts as empty: wrong offsets give wrong rows, never an access out of range.
 #pragma once
@@ -463,7 +465,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             // are written again only after the MMAs that read them have freed the stage.  Columns: A's two
             // tiles of 128 elements, then per tile of 128 elements B's tile rows side by side (column j
             // holds rows 32 j ...).  (Copied by another thread, with a barrier between, a stage waits for
-            // the copies' completion: 43.7 us where this takes 39.4 for 4096^3.)
+            // the copies' completion: 4096^3 took 43.7 us so and 39.4 this way, when it was tried.)
             ta = sf_tmem + stage * sf_cols;
             tb = ta + 8u;
             const uint32_t sf = sSF + stage * sf_bytes;
@@ -706,7 +708,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       } else {
         // All of them to registers, rounded and in pairs (columns 2 j and 2 j + 1 of a chunk in word j), and the
         // accumulator back, before anything is stored: a tile of 256 columns has no second accumulator beside
-        // the scales, and the MMA warp would wait for the stores (4096^3 in 4 bits 37.8 us, 34.6 so).
+        // the scales, and the MMA warp would wait for the stores (4096^3 in 4 bits 37.8 us, 34.6 so, in short loops).
         uint32_t h[kChunks][16];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
@@ -733,7 +735,7 @@ hb_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // bytes, 16-byte pieces xor-swizzled by row pair.  Neighbouring lanes exchange halves first, so that
         // a lane stores the values of two features of one column (even lanes the even column): 128 bytes a
         // store without a bank conflict.  The MMA's operands come through the same shared memory.  (Two-byte
-        // stores to shared memory: 39.4 us where this takes 37.3; two-byte stores to memory: 45.)
+        // stores to shared memory took 39.4 us, this 37.3, two-byte stores to memory 45, when they were tried.)
         const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
         const uint32_t pair_base = stage_base + (lane & 1) * 64 + ((lane >> 1) & 3) * 4;
         const int piece = lane & 3;

@@ -1,5 +1,5 @@
 // Plans for the products grouped by expert and the 4-bit products (hb_group.cuh), and the launches of
-// the quantisation kernels (hb_mx.cuh).
+// the quantisation kernels (hb_mx.cuh).  Times at the rules are of loops of some 10 ms where nothing else is said.
 #pragma once
 #include "hb_plan.cuh"
 
@@ -83,9 +83,11 @@ void group_knobs(const GroupProblem& g, const hb_knobs* in, int sms, hb_knobs* o
   if (k.split_k == 0) {
     // A product of few tiles: the reduction of a tile over a cluster of 2 or 4 CTAs, as long as all of them
     // find an SM.  A tile's time is that of its operands through one SM's ring; the cluster costs about 2 us.
-    // Measured, one against four CTAs a tile: 64 rows x 4096 features, bf16, K 4096 17.6 / 14.5 us, 32 rows
-    // 18.5 / 12.1; MXFP4 32 rows, K 8192 15.1 / 11.4, K 4096 (16 blocks) 9.6 / 10.0.  (Clusters of eight: 128
-    // CTAs did not all run at once, 12.3 us where four took 7.8.)
+    // Measured, one / two / four CTAs a tile, 32 rows x 4096 features in one group: bf16, K 4096 18.8 / 15.2 / 12.6 us;
+    // MXFP4, K 8192 14.3 / 13.4 / 11.4, K 4096 (16 blocks) 8.9 / 10.0 / 9.0.  (Clusters of eight: 128 CTAs did not all run
+    // at once, 12.3 us where four took 7.8.)  49 to 64 rows take tiles of 128 columns and no cluster, 18.0 us for 64 rows
+    // bf16, K 4096, although 64 columns and four CTAs take 14.7: most_tiles has to hold for all offsets and counts two
+    // tiles there.
     k.split_k = 1;
     if ((g.mode == hb::kFwd || g.mode == hb::kMx) && k.cta_group == 1 && k.tile_n == 64) {
       const int elems = g.mode == hb::kMx ? 256 : 64;

@@ -2,7 +2,7 @@
 // decoding step).  Such a product is one pass over the weights, 2 K N bytes an expert (16-bit) or K N (1/2 +
 // 1/32) (MXFP4), and the time is the memory's.  The tile kernel (hb_group.cuh) gives a tile of 128 features to
 // one SM, which draws at most about 50 bytes a cycle through its ring: with fewer tiles than SMs most of
-// the memory's bandwidth is idle (one token through 1024 x 2048 bf16: 9.9 us).  Here a block takes 16
+// the memory's bandwidth is idle (one token, 2048 features x 1024, bf16: 6.4 us by tiles, 3.2 here).  Here a block takes 16
 // features and up to eight rows of a group, its eight warps a share of the reduction each: every lane
 // loads its operands straight from memory in 16-byte pieces, many in flight before the first is used, and
 // the partial sums are joined in shared memory in the order of the warps.

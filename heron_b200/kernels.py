@@ -817,7 +817,8 @@ def quantize_mxfp4(x, offsets=None, codes=None, scales=None):
 
 
 def dequantize_mxfp4(codes, scales, offsets=None, out=None, out_dtype=None):
-    """The values that quantize_mxfp4's result stands for, float32 (default), bfloat16 or float16."""
+    """The values that quantize_mxfp4's result stands for, float32 (default), bfloat16 or float16.  With `offsets`, those of
+    the quantisation, rows of no group are left as they are in `out` (arbitrary in a fresh one)."""
     done = _fast.dequantize(codes, scales, offsets, out, out_dtype)
     if done is not None:
         return _done(done, "hb_dequantize_mxfp4")
